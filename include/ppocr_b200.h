@@ -548,6 +548,168 @@ int ppocr_engine_pool_recognize_batch(ppocr_engine_pool* pool, size_t count, con
 int ppocr_selftest_dispatch(size_t workers, size_t items, uint32_t stall_mask, uint32_t fail_mask, int stall_ms,
                             int timeout_ms, int* owner, int* values);
 
+/* ------------------------------------------------------------------------
+ * Sequence operators (new): attention over packed sequences, an 8-bit paged
+ * key / value cache with its single-token attention, and logit rules, on
+ * device memory that the caller owns.
+ *
+ * Every call enqueues one kernel (none for an empty input) on `stream` (a
+ * cudaStream_t of the handle's device; NULL = the handle's own stream, as in
+ * ppocr_model_run; the legacy default stream is passed as cudaStreamLegacy)
+ * and returns.  They allocate nothing, use no workspace and keep no state in
+ * the handle, so they may be captured into CUDA graphs, run on several
+ * streams at once and be called from several threads.  The calling thread's
+ * current device is left as it was.  Outputs must not overlap inputs, except
+ * where a call says so.
+ *
+ * Sizes, strides (in elements; the last axis is contiguous), types and
+ * pointers are checked by the call (PPOCR_ERR_INVALID_INPUT).  Offsets,
+ * lengths, block tables, ids and states live on the device, so the kernels
+ * check them: a bad one is never followed out of bounds, what it stands for
+ * is left out, and the next ppocr_gpu_synchronize reports it. */
+enum ppocr_dtype { PPOCR_DTYPE_F32 = 0, PPOCR_DTYPE_BF16 = 1 };
+
+/* A device tensor [tokens][heads][d]. */
+typedef struct ppocr_tokens {
+    void* data;
+    int64_t token_stride, head_stride;
+} ppocr_tokens;
+
+/* Waits (bounded by timeout_ms; <= 0: 60 s) for `stream` (NULL: the handle's
+ * own), then raises and clears what the sequence operators reported since the
+ * last call: PPOCR_ERR_INVALID_INPUT for a bad offset, length, table entry, id
+ * or state, PPOCR_ERR_GPU for a tensor-core pipeline wait that ran out. */
+int ppocr_gpu_synchronize(ppocr_gpu* gpu, void* stream, int timeout_ms);
+
+/* Attention over packed sequences: sequence i's queries are the tokens
+ * [q_offsets[i], q_offsets[i + 1]) of q, its keys and values the tokens
+ * [k_offsets[i], k_offsets[i + 1]) of k and v.  Query head h uses KV head
+ * h / (heads / kv_heads).
+ *   out = softmax(scale q k^T) v over the sequence's keys; causal: query j of
+ *   a sequence of nq queries and nk keys sees keys 0 .. j + nk - nq.
+ * A query that sees no key, or whose scores are all -infinity, gives zeros.
+ * Masked keys and values never reach an output, whatever they hold.  Tokens of
+ * `out` outside every sequence are left as they were.  d: 1..128; heads a
+ * multiple of kv_heads; scale > 0 (0: d^-1/2).  The recognizers' encoder
+ * attention (src/cpu/model.rs:1705-1725) is the case of equal lengths. */
+typedef struct ppocr_attention_packed_args {
+    int dtype;                   /* enum ppocr_dtype of q, k, v and out */
+    int heads, kv_heads, d;
+    int causal;                  /* 0 or 1 */
+    float scale;
+    int64_t sequences, total_q, total_k;
+    ppocr_tokens q, k, v, out;
+    const int32_t* q_offsets;    /* device, [sequences + 1] */
+    const int32_t* k_offsets;
+} ppocr_attention_packed_args;
+int ppocr_attention_packed(ppocr_gpu* gpu, const ppocr_attention_packed_args* args, void* stream);
+
+/* The cache: k and v are device arrays [pages][kv_heads][page][d] of integers
+ * in [-127, 127], k_scales and v_scales device arrays [pages][kv_heads]; slot
+ * s of head h of a page holds the value integer x scale.  16-byte aligned.
+ * page (tokens): 16, 32, 64 or 128; d: a multiple of 8 up to 128. */
+typedef struct ppocr_paged_cache {
+    int8_t* k;
+    int8_t* v;
+    float* k_scales;
+    float* v_scales;
+    int pages, kv_heads, page, d;
+} ppocr_paged_cache;
+
+/* pages[i * stride + b]: the page that holds tokens [b page, (b + 1) page) of
+ * sequence i.  Entries past a sequence's tokens are not read. */
+typedef struct ppocr_block_table {
+    const int32_t* pages;        /* device, [sequences][width] */
+    int64_t stride;
+    int sequences, width;        /* sequences * kv_heads at most 2^30 */
+} ppocr_block_table;
+
+/* Appends the tokens [offsets[i], offsets[i + 1]) of k and v to sequence i,
+ * which holds held[i] tokens.  A page's scale per head is the largest
+ * magnitude it has seen / 127: where new tokens raise the scale of a
+ * part-filled page, the integers it holds are rounded again.  A page's first
+ * token starts it afresh, whatever it held.  Integers are round(value / scale)
+ * of the exact quotient, ties to even; a value that is not finite makes its
+ * page's scale so.  A page being appended to belongs to one sequence; the
+ * lengths are the caller's to advance. */
+typedef struct ppocr_cache_append_args {
+    int dtype;                   /* of k and v */
+    int64_t total;               /* tokens of k and v */
+    ppocr_paged_cache cache;
+    ppocr_block_table table;
+    ppocr_tokens k, v;           /* [total][kv_heads][d] */
+    const int32_t* offsets;      /* device, [sequences + 1] */
+    const int32_t* held;         /* device, [sequences] */
+} ppocr_cache_append_args;
+int ppocr_cache_append(ppocr_gpu* gpu, const ppocr_cache_append_args* args, void* stream);
+
+/* Reads back, as values, the tokens first[i] .. of sequence i into the tokens
+ * [offsets[i], offsets[i + 1]) of k and v (ppocr_attention_packed over a
+ * prefix that only the cache holds). */
+typedef struct ppocr_cache_read_args {
+    int dtype;                   /* of k and v */
+    int64_t total;
+    ppocr_paged_cache cache;
+    ppocr_block_table table;
+    ppocr_tokens k, v;           /* outputs, [total][kv_heads][d] */
+    const int32_t* offsets;      /* device, [sequences + 1] */
+    const int32_t* first;        /* device, [sequences] */
+} ppocr_cache_read_args;
+int ppocr_cache_read(ppocr_gpu* gpu, const ppocr_cache_read_args* args, void* stream);
+
+/* Single-token attention: one query per sequence over the first lengths[i]
+ * tokens of its pages; a length of 0 gives zeros.  q and out are
+ * [sequences][heads][d]; scale as in ppocr_attention_packed. */
+typedef struct ppocr_attention_cached_args {
+    int dtype;                   /* of q and out */
+    int heads;
+    float scale;
+    ppocr_paged_cache cache;
+    ppocr_block_table table;
+    ppocr_tokens q, out;
+    const int32_t* lengths;      /* device, [sequences] */
+} ppocr_attention_cached_args;
+int ppocr_attention_cached(ppocr_gpu* gpu, const ppocr_attention_cached_args* args, void* stream);
+
+/* Logit rules: out[row] = the row's logits after, in this order,
+ *   repetition[row] r: ids in the row's history become x / r (x > 0) or x r;
+ *   - frequency[row] x count - presence[row] for ids with count > 0;
+ *   + bias[class];
+ *   -infinity where the row's mask has a 0 bit.
+ * Row i's history is the ids history[history_offsets[i] ..
+ * history_offsets[i + 1]).  Mask: bit c % 32 of word c / 32 allows class c;
+ * row i uses mask row mask_index[i] (-1: unmasked), or mask row 0 when
+ * mask_index is NULL.  NULL leaves a rule out; the penalties need a history.
+ * `out` may be `logits` (with the same stride). */
+typedef struct ppocr_logit_rules_args {
+    int dtype;                   /* of logits and out */
+    int rows, vocab, states;     /* states: mask rows */
+    const void* logits;          /* device, [rows][vocab] */
+    void* out;
+    int64_t stride, out_stride;  /* elements between rows */
+    const int32_t* history;
+    const int32_t* history_offsets;   /* device, [rows + 1] */
+    int64_t history_total;
+    const float* repetition;     /* device, [rows] */
+    const float* presence;
+    const float* frequency;
+    const float* bias;           /* device, [vocab] */
+    const uint32_t* mask;        /* device, [states][mask_stride >= ceil(vocab / 32)] */
+    int64_t mask_stride;
+    const int32_t* mask_index;   /* device, [rows] */
+} ppocr_logit_rules_args;
+int ppocr_logit_rules(ppocr_gpu* gpu, const ppocr_logit_rules_args* args, void* stream);
+
+/* Recognizer only: ppocr_recognizer_forward_ctc held to the caller's classes.
+ * `bias` (host, `classes` finite values, or NULL) is added to every step's
+ * logits; `allowed` (host, ceil(classes / 32) words, bit c % 32 of word c / 32,
+ * at least one class set, or NULL) leaves the other classes out, as the blank
+ * class unless its bit is set.  The probabilities are over the allowed
+ * classes; with a single one the margin is FLT_MAX. */
+int ppocr_recognizer_forward_ctc_rules(ppocr_model* model, const float* input, size_t input_len, const float* bias,
+                                       const uint32_t* allowed, int32_t* indices, float* probabilities,
+                                       float* margins);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,7 @@
 
 #include "common.hpp"
 #include "handles.hpp"
+#include "../kernels/seq.h"
 #include "models.hpp"
 #include "ppocr_b200.h"
 #include "safetensors.hpp"
@@ -142,11 +143,13 @@ struct ppocr_model {
     int* dflags = nullptr;   // device flags (kFlags ints, see above)
     int* hflags = nullptr;   // pinned host copy
     int* dcounters = nullptr;   // the plan's fused-SE arrival counters (zero between launches)
+    void* drules = nullptr;     // bias and class mask of ppocr_recognizer_forward_ctc_rules
 
     ~ppocr_model() {
         if (exec) cudaGraphExecDestroy(exec);
         if (dflags) cudaFree(dflags);
         if (dcounters) cudaFree(dcounters);
+        if (drules) cudaFree(drules);
         PinnedFlags::release(hflags);
     }
 
@@ -351,6 +354,7 @@ void ppocr::gpu_release(ppocr_gpu* gpu) {
     if (gpu->side) cudaStreamDestroy(gpu->side);
     if (gpu->fork) cudaEventDestroy(gpu->fork);
     if (gpu->join) cudaEventDestroy(gpu->join);
+    PinnedFlags::release(gpu->seq_status);
     delete gpu;
 }
 
@@ -402,6 +406,9 @@ int ppocr_gpu_create(int device, ppocr_gpu** out) {
         cuda_check(cudaStreamCreateWithFlags(&g->side, cudaStreamNonBlocking), "create side stream");
         cuda_check(cudaEventCreateWithFlags(&g->fork, cudaEventDisableTiming), "create fork event");
         cuda_check(cudaEventCreateWithFlags(&g->join, cudaEventDisableTiming), "create join event");
+        static_assert(kSeqStatusWords <= (int)kFlags, "the status words come from the pinned flag sets");
+        g->seq_status = PinnedFlags::acquire();
+        std::fill_n(g->seq_status, kFlags, 0);
         *out = g.release();
     });
 }
@@ -1703,6 +1710,59 @@ int ppocr_selftest_engine(ppocr_gpu* gpu, int planes, int n, int hi, int wi, int
         if (used_tensor_cores) *used_tensor_cores = tc ? 1 : 0;
         const int err = tc_engine_error_and_clear();
         if (wait_error) *wait_error = err;
+    });
+}
+
+int ppocr_recognizer_forward_ctc_rules(ppocr_model* model, const float* input, size_t input_len, const float* bias,
+                                       const uint32_t* allowed, int32_t* indices, float* probabilities, float* margins) {
+    return guard([&] {
+        if (!model) fail(PPOCR_ERR_INVALID_INPUT, "model is null");
+        if (model->m.kind != Kind::Recognizer) fail(PPOCR_ERR_INVALID_INPUT, "CTC decode needs a recognizer");
+        const size_t classes = (size_t)model->m.classes, words = (classes + 31) / 32;
+        if (bias && !std::all_of(bias, bias + classes, [](float b) { return std::isfinite(b); }))
+            fail(PPOCR_ERR_INVALID_INPUT, "invalid input: class biases must be finite");
+        if (allowed) {
+            bool any = false;
+            for (size_t c = 0; c < classes && !any; ++c) any = (allowed[c / 32] >> (c % 32)) & 1u;
+            if (!any) fail(PPOCR_ERR_INVALID_INPUT, "invalid input: no class is allowed");
+        }
+        std::lock_guard<std::mutex> lock(model->gpu->mu);
+        model->gpu->bind();
+        cudaStream_t s = model->gpu->stream;
+        if (!model->drules) cuda_check(cudaMalloc(&model->drules, (classes + words) * 4), "allocate class rules");
+        float* dbias = static_cast<float*>(model->drules);
+        uint32_t* dmask = reinterpret_cast<uint32_t*>(dbias + classes);
+        if (bias) cuda_check(cudaMemcpyAsync(dbias, bias, classes * 4, cudaMemcpyHostToDevice, s), "upload class biases");
+        if (allowed) cuda_check(cudaMemcpyAsync(dmask, allowed, words * 4, cudaMemcpyHostToDevice, s), "upload allowed classes");
+        upload_and_run(model, input, input_len);
+        const size_t rows = (size_t)model->m.n * model->m.t;
+        // The forward's own output is checked before the rules can hide any of it.
+        cuda_check(launch_check_finite(static_cast<const float*>(model->tensor(model->m.probs)), model->m.output_elements,
+                                       model->dflags + 1, s),
+                   "check output");
+        LogitRulesParams r;
+        r.logits = r.out = model->tensor(model->m.logits);
+        r.ld = r.out_ld = model->m.logits_ld;
+        r.rows = (int)rows;
+        r.vocab = model->m.classes;
+        r.bias = bias ? dbias : nullptr;
+        r.mask = allowed ? dmask : nullptr;
+        r.mask_ld = (long long)words;
+        r.states = 1;
+        if (bias || allowed) cuda_check(launch_logit_rules(r, s), "apply class rules");
+        SoftmaxParams p;
+        p.rows = (int)rows;
+        p.classes = model->m.classes;
+        p.ld = model->m.logits_ld;
+        p.logits = static_cast<const float*>(model->tensor(model->m.logits));
+        p.index = static_cast<int32_t*>(model->tensor(model->m.index));
+        p.max_prob = static_cast<float*>(model->tensor(model->m.max_prob));
+        p.margin = static_cast<float*>(model->tensor(model->m.margin));
+        cuda_check(launch_softmax_ctc(p, s), "class statistics");
+        if (indices) download(model, model->m.index, indices, rows * 4);
+        if (probabilities) download(model, model->m.max_prob, probabilities, rows * 4);
+        if (margins) download(model, model->m.margin, margins, rows * 4);
+        finish(model, -1, 0);
     });
 }
 

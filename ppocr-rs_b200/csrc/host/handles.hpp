@@ -63,6 +63,9 @@ struct ppocr_gpu {
     size_t arena_bytes = 0;
     uint64_t arena_gen = 0;
     std::string name;
+    // What the sequence operators' kernels report (kSeqStatusWords ints of
+    // page-locked host memory that they write directly; see kernels/seq.h).
+    int* seq_status = nullptr;
 
     void bind() const {
         if (poisoned)

@@ -2,6 +2,7 @@
 // small conversion kernels.  Reference semantics are cited per kernel.
 #include "common.cuh"
 #include "kernels.h"
+#include "seq.h"
 
 #include <cfloat>
 
@@ -839,8 +840,27 @@ cudaError_t launch_layernorm(const LayerNormParams& p, cudaStream_t stream) {
 
 cudaError_t launch_attention(const AttentionParams& p, cudaStream_t stream) {
     const int warps = 4;
-    const size_t smem = (size_t)(2 * p.t * p.d + warps * p.d + warps * p.t) * sizeof(float);
-    if (smem > 200 * 1024) return cudaErrorInvalidValue;
+    const size_t smem = ((size_t)2 * p.t * p.d + (size_t)warps * p.d + (size_t)warps * p.t) * sizeof(float);
+    if (smem > 200 * 1024) {
+        // K and V of a line no longer fit in shared memory: the packed
+        // attention over n sequences of t tokens streams them.
+        const size_t e = dtype_size(p.dtype);
+        const char* qkv = static_cast<const char*>(p.qkv);
+        const long long hidden = (long long)p.heads * p.d;
+        PackedAttentionParams a;
+        a.q = {const_cast<char*>(qkv), 3 * hidden, p.d};
+        a.k = {const_cast<char*>(qkv) + hidden * e, 3 * hidden, p.d};
+        a.v = {const_cast<char*>(qkv) + 2 * hidden * e, 3 * hidden, p.d};
+        a.out = {p.out, hidden, p.d};
+        a.sequences = p.n;
+        a.uniform = p.t;
+        a.total_q = a.total_k = p.n * p.t;
+        a.heads = a.kv_heads = p.heads;
+        a.d = p.d;
+        a.scale = p.scale;
+        a.dtype = p.dtype;
+        return launch_attention_packed(a, stream);
+    }
     {
         cudaError_t e = p.dtype == DT_F32
             ? allow_dynamic_smem(reinterpret_cast<const void*>(attention_kernel<float>), 200 * 1024)

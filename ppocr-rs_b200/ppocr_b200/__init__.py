@@ -22,6 +22,7 @@ __all__ = [
     "TensorSizeOverflow", "TensorByteLength", "InvalidTensorRange", "InvalidModel", "InvalidInput", "GpuError",
     "ModelSize", "Precision", "Gpu", "GpuImage", "ImagePreprocess", "ModelOutput", "Detector", "Recognizer",
     "library", "library_path", "gpu_count", "inspect_model", "Engine", "EnginePool", "selftest_dispatch",
+    "DeviceArray", "PagedCache",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -137,6 +138,45 @@ class _LoadOptions(C.Structure):
                 ("reserved", C.c_int * 4)]
 
 
+class _Tokens(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class _AttentionPackedArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("heads", C.c_int), ("kv_heads", C.c_int), ("d", C.c_int), ("causal", C.c_int),
+                ("scale", C.c_float), ("sequences", C.c_int64), ("total_q", C.c_int64), ("total_k", C.c_int64),
+                ("q", _Tokens), ("k", _Tokens), ("v", _Tokens), ("out", _Tokens), ("q_offsets", C.c_void_p),
+                ("k_offsets", C.c_void_p)]
+
+
+class _PagedCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+                ("pages", C.c_int), ("kv_heads", C.c_int), ("page", C.c_int), ("d", C.c_int)]
+
+
+class _BlockTable(C.Structure):
+    _fields_ = [("pages", C.c_void_p), ("stride", C.c_int64), ("sequences", C.c_int), ("width", C.c_int)]
+
+
+class _CacheTokensArgs(C.Structure):
+    """ppocr_cache_append_args and ppocr_cache_read_args (the last field is `held` / `first`)."""
+    _fields_ = [("dtype", C.c_int), ("total", C.c_int64), ("cache", _PagedCache), ("table", _BlockTable), ("k", _Tokens),
+                ("v", _Tokens), ("offsets", C.c_void_p), ("positions", C.c_void_p)]
+
+
+class _AttentionCachedArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("heads", C.c_int), ("scale", C.c_float), ("cache", _PagedCache),
+                ("table", _BlockTable), ("q", _Tokens), ("out", _Tokens), ("lengths", C.c_void_p)]
+
+
+class _LogitRulesArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("rows", C.c_int), ("vocab", C.c_int), ("states", C.c_int), ("logits", C.c_void_p),
+                ("out", C.c_void_p), ("stride", C.c_int64), ("out_stride", C.c_int64), ("history", C.c_void_p),
+                ("history_offsets", C.c_void_p), ("history_total", C.c_int64), ("repetition", C.c_void_p),
+                ("presence", C.c_void_p), ("frequency", C.c_void_p), ("bias", C.c_void_p), ("mask", C.c_void_p),
+                ("mask_stride", C.c_int64), ("mask_index", C.c_void_p)]
+
+
 _SIZE4 = C.c_size_t * 4
 _lib = None
 
@@ -234,6 +274,13 @@ def library() -> C.CDLL:
                                                   C.POINTER(C.c_int)]),
         "ppocr_selftest_dispatch": (I, [S, S, C.c_uint32, C.c_uint32, I, I, C.POINTER(C.c_int),
                                         C.POINTER(C.c_int)]),
+        "ppocr_gpu_synchronize": (I, [P, P, I]),
+        "ppocr_attention_packed": (I, [P, C.POINTER(_AttentionPackedArgs), P]),
+        "ppocr_cache_append": (I, [P, C.POINTER(_CacheTokensArgs), P]),
+        "ppocr_cache_read": (I, [P, C.POINTER(_CacheTokensArgs), P]),
+        "ppocr_attention_cached": (I, [P, C.POINTER(_AttentionCachedArgs), P]),
+        "ppocr_logit_rules": (I, [P, C.POINTER(_LogitRulesArgs), P]),
+        "ppocr_recognizer_forward_ctc_rules": (I, [P, FP, S, FP, C.POINTER(C.c_uint32), C.POINTER(C.c_int32), FP, FP]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -277,6 +324,60 @@ def inspect_model(path: str, kind: str, size, input_shape: Sequence[int], precis
     rank = 4 if kind == "det" else 3
     return {"ops": ops.value, "arena_bytes": arena.value, "weight_bytes": wbytes.value,
             "output_shape": [int(v) for v in list(out)[:rank]]}
+
+
+# ---------------------------------------------------------------------------
+# Device arrays of the sequence operators
+# ---------------------------------------------------------------------------
+
+
+class DeviceArray:
+    """A device array by its address, shape, element type ("f32", "bf16", "i32", "u32" or "i8"), strides in
+    elements (None: contiguous) and device ordinal.  The sequence operators take this or anything that answers
+    as it does: ``data_ptr()``, ``shape``, ``stride()``, ``dtype`` and ``get_device()`` (a torch CUDA tensor)."""
+
+    def __init__(self, ptr: int, shape: Sequence[int], dtype: str, strides: Optional[Sequence[int]] = None,
+                 device: int = 0):
+        self.shape = tuple(int(v) for v in shape)
+        self.dtype = dtype
+        if strides is None:
+            step, out = 1, []
+            for v in reversed(self.shape):
+                out.append(step)
+                step *= v
+            strides = out[::-1]
+        self._ptr, self._strides, self._device = int(ptr), tuple(int(v) for v in strides), int(device)
+
+    def data_ptr(self) -> int:
+        return self._ptr
+
+    def stride(self):
+        return self._strides
+
+    def get_device(self) -> int:
+        return self._device
+
+
+@dataclass
+class PagedCache:
+    """The 8-bit paged key / value cache of ppocr_paged_cache: k and v are int8 device arrays
+    [pages, kv_heads, page, d], their scales FP32 device arrays [pages, kv_heads], all contiguous."""
+    k: object
+    v: object
+    k_scales: object
+    v_scales: object
+
+
+_DTYPES = {"f32": "f32", "bf16": "bf16", "i32": "i32", "u32": "i32", "i8": "i8", "torch.float32": "f32",
+           "torch.bfloat16": "bf16", "torch.int32": "i32", "torch.uint32": "i32", "torch.int8": "i8"}
+_dtype_names: dict = {}
+
+
+def _dtype_name(dtype) -> str:
+    name = _dtype_names.get(dtype)
+    if name is None:
+        name = _dtype_names[dtype] = _DTYPES.get(str(dtype), str(dtype))
+    return name
 
 
 # ---------------------------------------------------------------------------
@@ -467,6 +568,168 @@ class Gpu:
         _check(library().ppocr_selftest_conv_split(self._h, n, hi, wi, cin, cout, kh, kw, int(stride), int(pad), _fptr(x),
                                                    _fptr(w), None if b is None else _fptr(b), int(act),
                                                    None if r is None else _fptr(r), _fptr(out)))
+        return out
+
+    # -- sequence operators ---------------------------------------------------
+    # Arrays are DeviceArray or torch CUDA tensors on this device.  `stream` is None (the handle's own stream), a
+    # cudaStream_t as an integer (0: the legacy default stream) or an object with a `cuda_stream` (torch.cuda.Stream).
+    # The calls return after enqueueing; the arrays must stay alive until the stream has passed them.
+
+    def synchronize(self, stream=None, timeout_ms: int = 0) -> None:
+        """Waits for the stream, then raises what the sequence operators reported (ppocr_gpu_synchronize)."""
+        _check(library().ppocr_gpu_synchronize(self._h, self._stream(stream), int(timeout_ms)))
+
+    @staticmethod
+    def _stream(stream):
+        if stream is None:
+            return None
+        return getattr(stream, "cuda_stream", stream) or 1   # 1: cudaStreamLegacy
+
+    def _array(self, a, what: str, dtype: str, rank: int):
+        """Shape and strides of a device array after the checks that only its owner's framework can answer."""
+        shape = a.shape
+        if len(shape) != rank:
+            raise InvalidInput(f"invalid input: {what} has {len(shape)} axes; expected {rank}")
+        if _dtype_name(a.dtype) != dtype:
+            raise InvalidInput(f"invalid input: {what} holds {_dtype_name(a.dtype)}; expected {dtype}")
+        if a.get_device() != self.device:
+            raise InvalidInput(f"invalid input: {what} is on device {a.get_device()}; this handle is on device {self.device}")
+        return shape, a.stride()
+
+    def _flat(self, a, what: str, dtype: str, shape):
+        """Address of a contiguous array of the given shape (None: absent)."""
+        if a is None:
+            return None
+        got, strides = self._array(a, what, dtype, len(shape))
+        if tuple(got) != tuple(shape):
+            raise InvalidInput(f"invalid input: {what} has shape {tuple(got)}; expected {tuple(shape)}")
+        step = 1
+        for n, s in zip(reversed(got), reversed(strides)):
+            if n > 1 and s != step:
+                raise InvalidInput(f"invalid input: {what} is not contiguous")
+            step *= n
+        return a.data_ptr()
+
+    def _tokens(self, a, what: str, dtype: str, shape):
+        """A [tokens, heads, d] array with a contiguous last axis; -1 in `shape` leaves an extent open."""
+        got, s = self._array(a, what, dtype, 3)
+        if any(w != -1 and g != w for g, w in zip(got, shape)):
+            raise InvalidInput(f"invalid input: {what} has shape {tuple(got)}; expected {tuple(shape)}")
+        if got[2] > 1 and s[2] != 1:
+            raise InvalidInput(f"invalid input: {what}'s last axis is not contiguous")
+        return _Tokens(a.data_ptr(), s[0], s[1])
+
+    @staticmethod
+    def _value_type(a, what: str):
+        name = _dtype_name(a.dtype)
+        if name not in ("f32", "bf16"):
+            raise InvalidInput(f"invalid input: {what} holds {name}; expected f32 or bf16")
+        return name, 0 if name == "f32" else 1
+
+    def _cache(self, cache: PagedCache) -> _PagedCache:
+        pages, heads, page, d = self._array(cache.k, "cache.k", "i8", 4)[0]
+        return _PagedCache(self._flat(cache.k, "cache.k", "i8", (pages, heads, page, d)),
+                           self._flat(cache.v, "cache.v", "i8", (pages, heads, page, d)),
+                           self._flat(cache.k_scales, "cache.k_scales", "f32", (pages, heads)),
+                           self._flat(cache.v_scales, "cache.v_scales", "f32", (pages, heads)), pages, heads, page, d)
+
+    def _table(self, table) -> _BlockTable:
+        (sequences, width), s = self._array(table, "table", "i32", 2)
+        if width > 1 and s[1] != 1:
+            raise InvalidInput("invalid input: table's last axis is not contiguous")
+        return _BlockTable(table.data_ptr(), s[0], sequences, width)
+
+    def attention_packed(self, q, k, v, q_offsets, k_offsets, out, causal: bool = False, scale: Optional[float] = None,
+                         stream=None):
+        """softmax(scale q k^T) v per sequence of packed tokens (ppocr_attention_packed): q and out
+        [total_q, heads, d], k and v [total_k, kv_heads, d], offsets int32 [sequences + 1]; returns out."""
+        name, dtype = self._value_type(q, "q")
+        total_q, heads, d = self._array(q, "q", name, 3)[0]
+        total_k, kv_heads = self._array(k, "k", name, 3)[0][:2]
+        sequences = self._array(q_offsets, "q_offsets", "i32", 1)[0][0] - 1
+        if sequences < 0:
+            raise InvalidInput("invalid input: q_offsets is empty")
+        args = _AttentionPackedArgs(dtype, heads, kv_heads, d, 1 if causal else 0, self._scale(scale), sequences, total_q,
+                                    total_k, self._tokens(q, "q", name, (total_q, heads, d)),
+                                    self._tokens(k, "k", name, (total_k, kv_heads, d)),
+                                    self._tokens(v, "v", name, (total_k, kv_heads, d)),
+                                    self._tokens(out, "out", name, (total_q, heads, d)),
+                                    self._flat(q_offsets, "q_offsets", "i32", (sequences + 1,)),
+                                    self._flat(k_offsets, "k_offsets", "i32", (sequences + 1,)))
+        _check(library().ppocr_attention_packed(self._h, C.byref(args), self._stream(stream)))
+        return out
+
+    @staticmethod
+    def _scale(scale) -> float:
+        if scale is None:
+            return 0.0   # the library's default, d^-1/2
+        if not scale > 0:
+            raise InvalidInput("invalid input: scale must be positive")
+        return float(scale)
+
+    def _cache_tokens(self, call, cache, k, v, offsets, positions, what, table, stream):
+        name, dtype = self._value_type(k, "k")
+        c, t = self._cache(cache), self._table(table)
+        total = self._array(k, "k", name, 3)[0][0]
+        args = _CacheTokensArgs(dtype, total, c, t, self._tokens(k, "k", name, (total, c.kv_heads, c.d)),
+                                self._tokens(v, "v", name, (total, c.kv_heads, c.d)),
+                                self._flat(offsets, "offsets", "i32", (t.sequences + 1,)),
+                                self._flat(positions, what, "i32", (t.sequences,)))
+        _check(call(self._h, C.byref(args), self._stream(stream)))
+
+    def cache_append(self, cache: PagedCache, k, v, offsets, held, table, stream=None) -> None:
+        """Appends packed tokens k and v [total, kv_heads, d] to the sequences' pages (ppocr_cache_append):
+        offsets int32 [sequences + 1], held int32 [sequences] tokens before, table int32 [sequences, width]."""
+        self._cache_tokens(library().ppocr_cache_append, cache, k, v, offsets, held, "held", table, stream)
+
+    def cache_read(self, cache: PagedCache, k, v, offsets, first, table, stream=None) -> None:
+        """Reads tokens first[i].. of each sequence back as values into packed k and v (ppocr_cache_read)."""
+        self._cache_tokens(library().ppocr_cache_read, cache, k, v, offsets, first, "first", table, stream)
+
+    def attention_cached(self, cache: PagedCache, q, lengths, table, out, scale: Optional[float] = None, stream=None):
+        """Single-token attention over the cache (ppocr_attention_cached): q and out [sequences, heads, d],
+        lengths int32 [sequences], table int32 [sequences, width]; returns out."""
+        name, dtype = self._value_type(q, "q")
+        c, t = self._cache(cache), self._table(table)
+        heads = self._array(q, "q", name, 3)[0][1]
+        shape = (t.sequences, heads, c.d)
+        args = _AttentionCachedArgs(dtype, heads, self._scale(scale), c, t, self._tokens(q, "q", name, shape),
+                                    self._tokens(out, "out", name, shape),
+                                    self._flat(lengths, "lengths", "i32", (t.sequences,)))
+        _check(library().ppocr_attention_cached(self._h, C.byref(args), self._stream(stream)))
+        return out
+
+    def logit_rules(self, logits, out, history=None, history_offsets=None, repetition=None, presence=None,
+                    frequency=None, bias=None, mask=None, mask_index=None, stream=None):
+        """Penalties over each row's history, class biases and grammar masks (ppocr_logit_rules): logits and out
+        [rows, vocab] (out may be logits), history packed int32 ids with offsets [rows + 1], penalties FP32 [rows],
+        bias FP32 [vocab], mask int32 words [states, >= ceil(vocab / 32)], mask_index int32 [rows]; returns out."""
+        name, dtype = self._value_type(logits, "logits")
+        (rows, vocab), s = self._array(logits, "logits", name, 2)
+        got, so = self._array(out, "out", name, 2)
+        if tuple(got) != (rows, vocab):
+            raise InvalidInput(f"invalid input: out has shape {tuple(got)}; expected {(rows, vocab)}")
+        if vocab > 1 and (s[1] != 1 or so[1] != 1):
+            raise InvalidInput("invalid input: the last axis of logits or out is not contiguous")
+        if (history is None) != (history_offsets is None):
+            raise InvalidInput("invalid input: history and history_offsets go together")
+        ids = 0 if history is None else self._array(history, "history", "i32", 1)[0][0]
+        states, words, mask_ptr = 0, 0, None
+        if mask is not None:
+            (states, n), sm = self._array(mask, "mask", "i32", 2)
+            if n < -(-vocab // 32) or (n > 1 and sm[1] != 1):
+                raise InvalidInput(f"invalid input: mask rows must be {-(-vocab // 32)} contiguous words or more")
+            words = sm[0] if states > 1 else max(sm[0], n)
+            mask_ptr = mask.data_ptr()
+        args = _LogitRulesArgs(dtype, rows, vocab, states, logits.data_ptr(), out.data_ptr(), s[0], so[0],
+                               self._flat(history, "history", "i32", (ids,)),
+                               self._flat(history_offsets, "history_offsets", "i32", (rows + 1,)), ids,
+                               self._flat(repetition, "repetition", "f32", (rows,)),
+                               self._flat(presence, "presence", "f32", (rows,)),
+                               self._flat(frequency, "frequency", "f32", (rows,)),
+                               self._flat(bias, "bias", "f32", (vocab,)), mask_ptr, words,
+                               self._flat(mask_index, "mask_index", "i32", (rows,)))
+        _check(library().ppocr_logit_rules(self._h, C.byref(args), self._stream(stream)))
         return out
 
     def close(self) -> None:
@@ -676,9 +939,9 @@ class Recognizer(_Model):
     @classmethod
     def load(cls, gpu: Gpu, path: str, size, input_shape: Sequence[int], precision="fp32",
              use_graph: bool = True, shared_weights: Optional["Recognizer"] = None,
-             simt_only: bool = False) -> "Recognizer":
+             simt_only: bool = False, keep_tensors: bool = False) -> "Recognizer":
         h = C.c_void_p()
-        o = _options(precision, use_graph, simt_only)
+        o = _options(precision, use_graph, simt_only, keep_tensors)
         _check(library().ppocr_recognizer_load_ex(gpu._h, str(path).encode(), ModelSize.parse(size),
                                                   _SIZE4(*input_shape), C.byref(o),
                                                   shared_weights._h if shared_weights is not None else None,
@@ -707,13 +970,29 @@ class Recognizer(_Model):
         _check(library().ppocr_recognizer_forward_logits(self._h, _fptr(x), x.size, _fptr(out), out.size))
         return out
 
-    def forward_ctc(self, values):
-        """Greedy-CTC statistics per step: (arg-max index, its probability, top-2 logit margin), each [n, t]."""
+    def forward_ctc(self, values, bias=None, allowed=None):
+        """Greedy-CTC statistics per step: (arg-max index, its probability, top-2 logit margin), each [n, t].
+        `bias` ([classes] floats) is added to every step's logits and `allowed` ([classes] truth values, the blank
+        class 0 among them) leaves the other classes out (ppocr_recognizer_forward_ctc_rules)."""
         x = self._input(values)
-        n, t = self.output_shape[0], self.output_shape[1]
+        n, t, classes = self.output_shape
         idx = np.empty((n, t), dtype=np.int32)
         prob = np.empty((n, t), dtype=np.float32)
         margin = np.empty((n, t), dtype=np.float32)
+        if bias is not None or allowed is not None:
+            if bias is not None:
+                bias = np.ascontiguousarray(bias, dtype=np.float32)
+            if allowed is not None:
+                allowed = np.asarray(allowed, dtype=bool)
+            for name, a in (("bias", bias), ("allowed", allowed)):
+                if a is not None and a.shape != (classes,):
+                    raise InvalidInput(f"invalid input: {name} has shape {a.shape}; expected {(classes,)}")
+            bits = None if allowed is None else np.packbits(np.pad(allowed, (0, -classes % 32)), bitorder="little")
+            _check(library().ppocr_recognizer_forward_ctc_rules(
+                self._h, _fptr(x), x.size, None if bias is None else _fptr(bias),
+                None if bits is None else bits.ctypes.data_as(C.POINTER(C.c_uint32)),
+                idx.ctypes.data_as(C.POINTER(C.c_int32)), _fptr(prob), _fptr(margin)))
+            return idx, prob, margin
         _check(library().ppocr_recognizer_forward_ctc(self._h, _fptr(x), x.size,
                                                       idx.ctypes.data_as(C.POINTER(C.c_int32)), _fptr(prob),
                                                       _fptr(margin)))
