@@ -229,8 +229,8 @@ int ppocr_attention_cached(ppocr_gpu* gpu, const ppocr_attention_cached_args* ar
         p.cache = cache_of(a.cache);
         p.table = table_of(a.table, p.cache);
         check_heads(a.heads, p.cache.kv_heads);
-        // The grid: sequences x up to 8 parts of a sequence.
-        require(p.table.sequences <= INT_MAX / 8, "too many sequences for one call");
+        // The grid: sequences x up to 16 parts of a sequence.
+        require(p.table.sequences <= INT_MAX / 16, "too many sequences for one call");
         p.heads = a.heads;
         p.scale = scale_of(a.scale, p.cache.d);
         require(p.table.sequences == 0 || a.lengths, "lengths pointer is null");

@@ -20,7 +20,7 @@
 // A warp owns every fourth tile of its block's token range and keeps its own
 // softmax state; the running maximum moves only when a score passes it by
 // more than 8 (weights up to 2^8), so most tiles need no reduction at all.
-// The range of a sequence is split over the blocks of a cluster (1 to 8) when
+// The range of a sequence is split over the blocks of a cluster (1 to 16) when
 // there are few sequences and heads; warps join through shared memory, blocks
 // through distributed shared memory, both in a fixed order: one launch, no
 // workspace.
@@ -35,8 +35,9 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps, kHeads = 8;
-constexpr int kTile = 16;             // tokens per tile
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kHeads = 8, kMaxSplits = 16;
+constexpr int kTile = 16;             // tokens per tile: within one page, whatever its size
+constexpr int kPair = 2;              // tiles that a warp takes at a time: two independent chains of products
 constexpr float kSlack = 8.f;         // log2 of the largest weight before the maximum moves
 constexpr float kWeightScale = 64.f;  // weights are held times 64: a larger range above FP16's subnormals
 
@@ -58,6 +59,11 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void add4(float (&a)[4], const float (&b)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] += b[i];
+}
+
 // Transposes an 8 x 8 matrix of FP16 held two columns per lane (row lane / 4).
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
@@ -65,70 +71,69 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     return y;
 }
 
-// BYTES bytes of a cache row into words; bytes at and past `live` (a multiple
-// of 8) read as 0.  V16: rows are 16-byte aligned, else 8.
-template <int BYTES, bool V16>
-__device__ __forceinline__ void load_row(const int8_t* p, int live, uint32_t* w) {
-    if constexpr (BYTES == 4) {
-        w[0] = live > 0 ? __ldg(reinterpret_cast<const uint32_t*>(p)) : 0u;
-    } else if constexpr (BYTES == 16 && V16) {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (live > 0) u = __ldg(reinterpret_cast<const uint4*>(p));
-        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-    } else {
+// A warp's ring of pairs of tiles in shared memory: per tile the 16 K rows, the
+// 16 V rows (DP bytes each, zeros past d) and the page's two scales.  16-byte
+// chunks are permuted within a row so that the reads below, which take
+// different rows at the same bytes, spread over the banks.
+template <int DP, bool FULL>
+struct Ring {
+    static constexpr int kStages = 2, kChunks = DP / 16, kRows = kTile * DP, kOne = 2 * kRows + 16, kStage = kPair * kOne;
+    static constexpr int kBytes = kStages * kStage;
+    static __device__ __forceinline__ int k_chunk(int row, int chunk) { return DP == 128 ? chunk ^ (row & 1) << 2 : chunk; }
+    static __device__ __forceinline__ int v_chunk(int row, int chunk) {
+        return DP == 128 ? chunk ^ (row >> 1 & 3) << 1 : DP == 64 ? chunk ^ (row >> 1 & 3) : chunk;
+    }
+
+    // Starts the copies of slots slot0 .. slot0 + 15 of `head` of page `where`.
+    static __device__ __forceinline__ void fetch(const CachedAttentionParams& p, uint32_t stage, int where, int head, int slot0,
+                                                 int lane) {
+        const int d = FULL ? DP : p.cache.d;
+        const long long cell = (long long)where * p.cache.kv_heads + head, at0 = (cell * p.cache.page + slot0) * d;
+        const int8_t* kp = p.cache.k + at0;
+        const int8_t* vp = p.cache.v + at0;
 #pragma unroll
-        for (int i = 0; i < BYTES / 8; ++i) {
-            uint2 u = make_uint2(0, 0);
-            if (8 * i < live) u = __ldg(reinterpret_cast<const uint2*>(p) + i);
-            w[2 * i] = u.x; w[2 * i + 1] = u.y;
+        for (int i = 0; i < kTile * kChunks / 32; ++i) {
+            const int row = (lane + 32 * i) / kChunks, chunk = (lane + 32 * i) % kChunks, from = row * d + chunk * 16;
+            const uint32_t to = stage + row * DP;
+            copy(to + k_chunk(row, chunk) * 16, kp + from, d - chunk * 16, kp);
+            copy(to + kRows + v_chunk(row, chunk) * 16, vp + from, d - chunk * 16, vp);
+        }
+        if (lane < 2) copy4(stage + 2 * kRows + 4 * lane, (lane ? p.cache.v_scales : p.cache.k_scales) + cell);
+    }
+    // 16 bytes of a row with `live` of them (a multiple of 8; FULL: all) in it.
+    static __device__ __forceinline__ void copy(uint32_t to, const int8_t* from, int live, const int8_t* base) {
+        if constexpr (FULL) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int n = live > 8 * h ? 8 : 0;
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to + 8 * h), "l"(n ? from + 8 * h : base), "r"(n) : "memory");
+            }
         }
     }
-}
-
-// Bytes of K that a lane holds of one token, by piece: values of d
-// [at, at + kPieceK) for piece 0, 64 further for piece 1.
-template <int DP> constexpr int kPieceK = DP == 32 ? 8 : 16;
-template <int DP> constexpr int kPiecesK = DP / 4 / kPieceK<DP>;
-
-template <int DP, bool V16>
-struct TileData {
-    uint32_t k[2][DP / 16];   // tokens lane / 4 and lane / 4 + 8
-    uint32_t v[4][DP / 32];   // tokens 2c, 2c + 1, 2c + 8, 2c + 9 with c = lane % 4
-    float sk, sv;
-    bool ok;
-
-    __device__ __forceinline__ void load(const CachedAttentionParams& p, int where, int head, int slot0, int lane) {
-        ok = where >= 0;
-        if (!ok) return;
-        const int d = p.cache.d, r = lane >> 2, c = lane & 3;
-        const long long cell = (long long)where * p.cache.kv_heads + head;
-        const int8_t* kp = p.cache.k + (cell * p.cache.page + slot0) * d;
-        const int8_t* vp = p.cache.v + (cell * p.cache.page + slot0) * d;
-        sk = __ldg(p.cache.k_scales + cell);
-        sv = __ldg(p.cache.v_scales + cell);
-        constexpr int PK = kPieceK<DP>;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < kPiecesK<DP>; ++i) {
-                const int at = 64 * i + c * PK;
-                load_row<PK, V16>(kp + (r + 8 * t) * d + at, d - at, &k[t][i * PK / 4]);
-            }
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int tok = 2 * c + (t & 1) + 8 * (t >> 1), at = r * (DP / 8);
-            load_row<DP / 8, V16>(vp + tok * d + at, d - at, v[t]);
-        }
+    static __device__ __forceinline__ void copy4(uint32_t to, const float* from) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
     }
 };
 
-template <typename T, int DP, bool V16>
-__global__ void __launch_bounds__(kThreads) attention_cached_kernel(CachedAttentionParams p, int splits) {
+// BYTES (4, 8 or 16) bytes of shared memory.
+template <int BYTES>
+__device__ __forceinline__ void read_words(uint32_t at, uint32_t* w) {
+    if constexpr (BYTES == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(at));
+    else if constexpr (BYTES == 8) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
+    else asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+}
+
+template <typename T, int DP, bool FULL>
+__global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAttentionParams p, int splits) {
     constexpr bool SPLIT = sizeof(T) == 4;   // FP32: two FP16 pieces
     constexpr int KS = DP / 16;              // 16-wide steps over d
-    constexpr int PK = kPieceK<DP>;
-    __shared__ float sm_o[kWarps][kHeads][DP];
-    __shared__ float sm_m[kWarps][kHeads], sm_l[kWarps][kHeads];
+    // A lane holds, of a token of K, the bytes at c PK (and, for d 128, 64
+    // further), of a token of V the bytes at r DP / 8.
+    constexpr int PK = DP == 32 ? 8 : 16, PV = DP / 8;
+    using Tiles = Ring<DP, FULL>;
+    extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     const int seq = blockIdx.x / splits, split = blockIdx.x % splits;
     const int group = p.heads / p.cache.kv_heads, parts = (group + kHeads - 1) / kHeads;
@@ -142,25 +147,45 @@ __global__ void __launch_bounds__(kThreads) attention_cached_kernel(CachedAttent
         if (threadIdx.x == 0) seq_bad_index(p.status);
         len = len < 0 ? 0 : (int)room;
     }
-    const int tiles = (len + kTile - 1) / kTile, per = (tiles + splits - 1) / splits;
-    const int t_end = min(tiles, (split + 1) * per);
+    // Pairs of tiles, dealt to the splits in ranges and to a block's warps by turns.
+    const int tiles = (len + kTile - 1) / kTile, pairs = (tiles + kPair - 1) / kPair, per = (pairs + splits - 1) / splits;
+    const int t_end = min(pairs, (split + 1) * per);
     const int32_t* pages = p.table.pages + seq * p.table.stride;
-    auto page_of = [&](int t) {
-        if (t >= t_end) return -1;
-        const int w = __ldg(pages + t * kTile / page);
-        if (w < 0 || w >= p.cache.pages) {
+    const int page_shift = 31 - __clz(page) - 4;   // log2 of the tiles in a page
+    auto page_of = [&](int pair, int half) {
+        const int tile = pair * kPair + half;
+        if (pair >= t_end || tile >= tiles) return -1;
+        const int w = __ldg(pages + (tile >> page_shift));
+        if ((unsigned)w >= (unsigned)p.cache.pages) {
             seq_bad_index(p.status);
             return -1;
         }
         return w;
     };
-    TileData<DP, V16> cur, nxt;
-    int t = split * per + warp;
-    {
-        const int w0 = page_of(t);
-        cur.load(p, w0, kv, t * kTile % page, lane);
-    }
-    int w_next = page_of(t + kWarps);
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * Tiles::kBytes;
+    int t = split * per + warp;      // the pair at hand
+    int ahead = t, stage = 0, stage_ahead = 0, w_ahead[kPair];   // the next pair to fetch and its pages
+    unsigned missing = 0;            // bit kPair s + h: half h of stage s holds no tile
+#pragma unroll
+    for (int h = 0; h < kPair; ++h) w_ahead[h] = page_of(ahead, h);
+    auto fetch = [&] {
+        missing &= ~(((1u << kPair) - 1) << kPair * stage_ahead);
+#pragma unroll
+        for (int h = 0; h < kPair; ++h) {
+            if (w_ahead[h] >= 0)
+                Tiles::fetch(p, ring + stage_ahead * Tiles::kStage + h * Tiles::kOne, w_ahead[h], kv,
+                             (ahead * kPair + h) * kTile & (page - 1), lane);
+            else
+                missing |= 1u << (kPair * stage_ahead + h);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        ahead += kWarps;
+#pragma unroll
+        for (int h = 0; h < kPair; ++h) w_ahead[h] = page_of(ahead, h);
+        stage_ahead = stage_ahead + 1 == Tiles::kStages ? 0 : stage_ahead + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < Tiles::kStages - 1; ++i) fetch();
 
     // B operand of the scores: head r's values of d, in the order in which the
     // lane's K bytes come; b0 holds bytes 4s, 4s + 1 and b1 bytes 4s + 2, 4s + 3.
@@ -203,82 +228,151 @@ __global__ void __launch_bounds__(kThreads) attention_cached_kernel(CachedAttent
     for (int j = 0; j < KS; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, ref = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    float b0 = 0.f, b1 = 0.f;        // m0 and m1, 0 where they are -infinity
+    float ref = 0.f, unit = 1.f;     // R, and what a V scale is multiplied by
 
+    const uint32_t k_at = r * DP, v_at = Tiles::kRows + 2 * c * DP;
     for (; t < t_end; t += kWarps) {
-        nxt.load(p, w_next, kv, (t + kWarps) * kTile % page, lane);
-        w_next = page_of(t + 2 * kWarps);
-        if (cur.ok) {
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
+        asm volatile("cp.async.wait_group %0;" ::"n"(Tiles::kStages - 2) : "memory");
+        __syncwarp();   // the pair is there, and every lane has read the one that the next copies replace
+        fetch();
+        const uint32_t at = ring + stage * Tiles::kStage;
+        const unsigned none = missing >> kPair * stage;
+        stage = stage + 1 == Tiles::kStages ? 0 : stage + 1;
+
+        // Scores: [tokens][heads] of each tile.  The tensor cores truncate when
+        // they add to an accumulator, so FP32 sums take few steps each: the
+        // second pieces apart (they are 2^-11 of the first), the first in
+        // chains of two steps.
+        float s[kPair][4], sv[kPair];
+#pragma unroll
+        for (int h = 0; h < kPair; ++h) {
+            uint32_t k[2][DP / 16];
+            float sk, rest[4] = {0.f, 0.f, 0.f, 0.f}, part[4];
+            asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(sk), "=f"(sv[h]) : "r"(at + h * Tiles::kOne + 2 * Tiles::kRows));
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < DP / 4 / PK; ++j)
+                    read_words<PK>(at + h * Tiles::kOne + k_at + 8 * i * DP + Tiles::k_chunk(r, (c * PK >> 4) + 4 * j) * 16 +
+                                       (c * PK & 15),
+                                   &k[i][j * PK / 4]);
+            s[h][0] = s[h][1] = s[h][2] = s[h][3] = 0.f;
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
-                const uint32_t u0 = cur.k[0][i] ^ 0x80808080u, u1 = cur.k[1][i] ^ 0x80808080u;
+                const uint32_t u0 = k[0][i] ^ 0x80808080u, u1 = k[1][i] ^ 0x80808080u;
                 const uint32_t a0 = bytes_to_h2(u0, 0x4140), a1 = bytes_to_h2(u1, 0x4140);
                 const uint32_t a2 = bytes_to_h2(u0, 0x4342), a3 = bytes_to_h2(u1, 0x4342);
-                mma_f16(s, a0, a1, a2, a3, qh[i][0], qh[i][1]);
-                if constexpr (SPLIT) mma_f16(s, a0, a1, a2, a3, ql[i][0], ql[i][1]);
-            }
-            const int tok = t * kTile + r;
-            const float k0 = f0 * cur.sk, k1 = f1 * cur.sk;
-            s[0] = tok < len ? s[0] * k0 : -INFINITY;
-            s[1] = tok < len ? s[1] * k1 : -INFINITY;
-            s[2] = tok + 8 < len ? s[2] * k0 : -INFINITY;
-            s[3] = tok + 8 < len ? s[3] * k1 : -INFINITY;
-            const float t0 = fmaxf(s[0], s[2]), t1 = fmaxf(s[1], s[3]);
-            if (__any_sync(0xffffffffu, t0 > m0 + kSlack || t1 > m1 + kSlack || cur.sv > 2.f * ref)) {
-                float n0 = fmaxf(t0, m0), n1 = fmaxf(t1, m1);
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) {
-                    n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
-                    n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
-                }
-                const float g0 = m0 == -INFINITY ? 0.f : exp2_hw(m0 - n0), g1 = m1 == -INFINITY ? 0.f : exp2_hw(m1 - n1);
-                const float next = fmaxf(ref, cur.sv);
-                const float back = next > ref ? ref / next : 1.f;
-                m0 = n0; m1 = n1; ref = next;
-                l0 *= g0; l1 *= g1;
-#pragma unroll
-                for (int j = 0; j < KS; ++j) {
-                    o[j][0] *= g0 * back; o[j][1] *= g1 * back;
-                    o[j][2] *= g0 * back; o[j][3] *= g1 * back;
+                if constexpr (SPLIT) {
+                    if (i % 2 == 0) part[0] = part[1] = part[2] = part[3] = 0.f;
+                    mma_f16(part, a0, a1, a2, a3, qh[i][0], qh[i][1]);
+                    mma_f16(rest, a0, a1, a2, a3, ql[i][0], ql[i][1]);
+                    if (i % 2 == 1) add4(s[h], part);
+                } else {
+                    mma_f16(s[h], a0, a1, a2, a3, qh[i][0], qh[i][1]);
                 }
             }
-            const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
-            s[0] = exp2_hw(s[0] - b0); s[1] = exp2_hw(s[1] - b1);
-            s[2] = exp2_hw(s[2] - b0); s[3] = exp2_hw(s[3] - b1);
-            l0 += s[0] + s[2];
-            l1 += s[1] + s[3];
-            // ref is 0 only while every V scale seen is 0: weights of zeros.
-            const float w = ref > 0.f ? cur.sv * (kWeightScale / ref) : cur.sv;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] *= w;
-            const __half2 h0 = __floats2half2_rn(s[0], s[1]), h1 = __floats2half2_rn(s[2], s[3]);
-            const uint32_t p0 = transpose8(h2_bits(h0)), p1 = transpose8(h2_bits(h1));
-            uint32_t e0 = 0, e1 = 0;
-            if constexpr (SPLIT) {
-                const float2 x = __half22float2(h0), y = __half22float2(h1);
-                e0 = transpose8(h2_bits(__floats2half2_rn(s[0] - x.x, s[1] - x.y)));
-                e1 = transpose8(h2_bits(__floats2half2_rn(s[2] - y.x, s[3] - y.y)));
-            }
-#pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                const uint32_t u0 = cur.v[0][i] ^ 0x80808080u, u1 = cur.v[1][i] ^ 0x80808080u;
-                const uint32_t u2 = cur.v[2][i] ^ 0x80808080u, u3 = cur.v[3][i] ^ 0x80808080u;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    // Bytes 2h and 2h + 1 of two tokens, interleaved by value of d.
-                    const uint32_t x = __byte_perm(u0, u1, h ? 0x7362 : 0x5140), y = __byte_perm(u2, u3, h ? 0x7362 : 0x5140);
-                    const uint32_t a0 = bytes_to_h2(x, 0x4140), a1 = bytes_to_h2(x, 0x4342);
-                    const uint32_t a2 = bytes_to_h2(y, 0x4140), a3 = bytes_to_h2(y, 0x4342);
-                    mma_f16(o[2 * i + h], a0, a1, a2, a3, p0, p1);
-                    if constexpr (SPLIT) mma_f16(o[2 * i + h], a0, a1, a2, a3, e0, e1);
-                }
+            if constexpr (SPLIT) add4(s[h], rest);
+            const float k0 = f0 * sk, k1 = f1 * sk;
+            s[h][0] *= k0; s[h][1] *= k1;
+            s[h][2] *= k0; s[h][3] *= k1;
+            // Past the sequence's end, or on a page that is none.
+            const int left = none >> h & 1 ? 0 : len - (t * kPair + h) * kTile;
+            if (left < kTile) {
+                if (r >= left) s[h][0] = s[h][1] = -INFINITY;
+                if (r + 8 >= left) s[h][2] = s[h][3] = -INFINITY;
+                if (left <= 0) sv[h] = 0.f;   // what the stage holds is older
             }
         }
-        cur = nxt;
+        float t0 = -INFINITY, t1 = -INFINITY, tv = 0.f;
+#pragma unroll
+        for (int h = 0; h < kPair; ++h) {
+            t0 = fmaxf(t0, fmaxf(s[h][0], s[h][2]));
+            t1 = fmaxf(t1, fmaxf(s[h][1], s[h][3]));
+            tv = fmaxf(tv, sv[h]);
+        }
+        if (__any_sync(0xffffffffu, t0 > m0 + kSlack || t1 > m1 + kSlack || tv > 2.f * ref)) {
+            float n0 = fmaxf(t0, m0), n1 = fmaxf(t1, m1);
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+                n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
+                n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
+            }
+            const float g0 = m0 == -INFINITY ? 0.f : exp2_hw(m0 - n0), g1 = m1 == -INFINITY ? 0.f : exp2_hw(m1 - n1);
+            const float next = fmaxf(ref, tv);
+            const float back = next > ref ? ref / next : 1.f;
+            m0 = n0; m1 = n1; ref = next;
+            b0 = m0 == -INFINITY ? 0.f : m0;
+            b1 = m1 == -INFINITY ? 0.f : m1;
+            unit = ref > 0.f ? kWeightScale / ref : 1.f;   // 0 only while every V scale seen is 0: weights of zeros
+            l0 *= g0; l1 *= g1;
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+                o[j][0] *= g0 * back; o[j][1] *= g1 * back;
+                o[j][2] *= g0 * back; o[j][3] *= g1 * back;
+            }
+        }
+        // Weights, as the B operand of the second product.
+        uint32_t p0[kPair], p1[kPair], e0[kPair], e1[kPair], v[kPair][4][DP / 32];
+#pragma unroll
+        for (int h = 0; h < kPair; ++h) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = (i & 1) + 8 * (i >> 1);
+                read_words<PV>(at + h * Tiles::kOne + v_at + row * DP + Tiles::v_chunk(2 * c, r * PV >> 4) * 16 + (r * PV & 15),
+                               v[h][i]);
+            }
+            float* x = s[h];
+            x[0] = exp2_hw(x[0] - b0); x[1] = exp2_hw(x[1] - b1);
+            x[2] = exp2_hw(x[2] - b0); x[3] = exp2_hw(x[3] - b1);
+            l0 += x[0] + x[2];
+            l1 += x[1] + x[3];
+            const float w = sv[h] * unit;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] *= w;
+            const __half2 h0 = __floats2half2_rn(x[0], x[1]), h1 = __floats2half2_rn(x[2], x[3]);
+            p0[h] = transpose8(h2_bits(h0));
+            p1[h] = transpose8(h2_bits(h1));
+            if constexpr (SPLIT) {
+                const float2 y = __half22float2(h0), z = __half22float2(h1);
+                e0[h] = transpose8(h2_bits(__floats2half2_rn(x[0] - y.x, x[1] - y.y)));
+                e1[h] = transpose8(h2_bits(__floats2half2_rn(x[2] - z.x, x[3] - z.y)));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < kPair; ++h) {
+                    // Bytes 2b and 2b + 1 of two tokens, interleaved by value of d.
+                    const uint32_t x = __byte_perm(v[h][0][i], v[h][1][i], b ? 0x7362 : 0x5140) ^ 0x80808080u;
+                    const uint32_t y = __byte_perm(v[h][2][i], v[h][3][i], b ? 0x7362 : 0x5140) ^ 0x80808080u;
+                    const uint32_t a0 = bytes_to_h2(x, 0x4140), a1 = bytes_to_h2(x, 0x4342);
+                    const uint32_t a2 = bytes_to_h2(y, 0x4140), a3 = bytes_to_h2(y, 0x4342);
+                    if constexpr (SPLIT) {   // a pair's sum apart, added to the running one with rounding
+                        mma_f16(sum, a0, a1, a2, a3, e0[h], e1[h]);
+                        mma_f16(sum, a0, a1, a2, a3, p0[h], p1[h]);
+                    } else {
+                        mma_f16(o[2 * i + b], a0, a1, a2, a3, p0[h], p1[h]);
+                    }
+                }
+                if constexpr (SPLIT) add4(o[2 * i + b], sum);
+            }
     }
 
-    // Join the warps, then the cluster's blocks.
+    // Join the block's warps, where the rings were: warp w's sums at sm_o[w],
+    // then their sum at sm_o[0], all taken relative to the block's maximum.
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    float (*sm_o)[kHeads][DP] = reinterpret_cast<float (*)[kHeads][DP]>(smem);
+    float (*sm_m)[kHeads] = reinterpret_cast<float (*)[kHeads]>(sm_o + kWarps);
+    float (*sm_l)[kHeads] = sm_m + kWarps;
+    float* top = reinterpret_cast<float*>(sm_l + kWarps);   // [kHeads], the block's maximum
+    float* sum = top + kHeads;                              // [kHeads], and sum
+    float* share = sum + kHeads;                            // [splits][kHeads]
 #pragma unroll
     for (int x = 4; x < 32; x <<= 1) {
         l0 += __shfl_xor_sync(0xffffffffu, l0, x);
@@ -288,52 +382,78 @@ __global__ void __launch_bounds__(kThreads) attention_cached_kernel(CachedAttent
         sm_m[warp][2 * c] = m0; sm_m[warp][2 * c + 1] = m1;
         sm_l[warp][2 * c] = l0; sm_l[warp][2 * c + 1] = l1;
     }
-    const float unit = ref > 0.f ? ref / kWeightScale : 1.f;
+    const float back = ref > 0.f ? ref / kWeightScale : 1.f;
 #pragma unroll
     for (int j = 0; j < KS; ++j) {
-        const int at = r * (DP / 8) + 2 * j;
-        sm_o[warp][2 * c][at] = o[j][0] * unit;
-        sm_o[warp][2 * c + 1][at] = o[j][1] * unit;
-        sm_o[warp][2 * c][at + 1] = o[j][2] * unit;
-        sm_o[warp][2 * c + 1][at + 1] = o[j][3] * unit;
+        const int x = r * (DP / 8) + 2 * j;
+        *reinterpret_cast<float2*>(&sm_o[warp][2 * c][x]) = make_float2(o[j][0] * back, o[j][2] * back);
+        *reinterpret_cast<float2*>(&sm_o[warp][2 * c + 1][x]) = make_float2(o[j][1] * back, o[j][3] * back);
     }
-    cg::cluster_group cluster = cg::this_cluster();
-    if (splits > 1) cluster.sync(); else __syncthreads();
-    // Outputs are dealt to the cluster's threads; each sums the warps of all
-    // blocks in order.
-    const int rank = splits > 1 ? (int)cluster.block_rank() : 0;
-    for (int i = rank * kThreads + threadIdx.x; i < live_heads * d; i += splits * kThreads) {
-        const int h = i / d, x = i % d;
-        float top = -INFINITY;
-        for (int b = 0; b < splits; ++b) {
-            const float* m = splits > 1 ? cluster.map_shared_rank(&sm_m[0][0], b) : &sm_m[0][0];
+    __syncthreads();
+    auto factor = [](float m, float most) { return m == -INFINITY ? 0.f : exp2_hw(m - most); };
+    for (int i = threadIdx.x; i < live_heads * DP; i += kThreads) {
+        const int h = i / DP, x = i % DP;
+        float most = sm_m[0][h];
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, m[w * kHeads + h]);
+        for (int w = 1; w < kWarps; ++w) most = fmaxf(most, sm_m[w][h]);
+        float a = 0.f, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float g = factor(sm_m[w][h], most);
+            a = fmaf(g, sm_o[w][h][x], a);
+            l = fmaf(g, sm_l[w][h], l);
         }
-        float sum = 0.f, l = 0.f;
-        for (int b = 0; b < splits; ++b) {
-            const float* m = splits > 1 ? cluster.map_shared_rank(&sm_m[0][0], b) : &sm_m[0][0];
-            const float* ls = splits > 1 ? cluster.map_shared_rank(&sm_l[0][0], b) : &sm_l[0][0];
-            const float* os = splits > 1 ? cluster.map_shared_rank(&sm_o[0][0][0], b) : &sm_o[0][0][0];
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float mw = m[w * kHeads + h];
-                const float g = mw == -INFINITY ? 0.f : exp2_hw(mw - top);
-                l = fmaf(g, ls[w * kHeads + h], l);
-                sum = fmaf(g, os[(w * kHeads + h) * DP + x], sum);
+        if (splits == 1) {
+            T* out = static_cast<T*>(p.out.ptr) + seq * p.out.token_stride + (head0 + h) * p.out.head_stride;
+            if (x < d) out[x] = from_f<T>(l == 0.f ? 0.f : a / l);
+        } else {
+            sm_o[0][h][x] = a;
+            if (x == 0) {
+                top[h] = most;
+                sum[h] = l;
             }
         }
-        T* out = static_cast<T*>(p.out.ptr) + seq * p.out.token_stride + (head0 + h) * p.out.head_stride;
-        out[x] = from_f<T>(l == 0.f ? 0.f : sum / l);
     }
-    if (splits > 1) cluster.sync();   // no block leaves while another reads its shared memory
+    if (splits == 1) return;
+
+    // Join the cluster's blocks: each one's share in a head's output, then the
+    // outputs, dealt to the cluster's threads, each summed in the blocks' order.
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    if (threadIdx.x < live_heads) {
+        const int h = threadIdx.x;
+        float most = -INFINITY, l = 0.f;
+        for (int b = 0; b < splits; ++b) most = fmaxf(most, *cluster.map_shared_rank(top + h, b));
+        for (int b = 0; b < splits; ++b) {
+            const float g = factor(*cluster.map_shared_rank(top + h, b), most);
+            share[b * kHeads + h] = g;
+            l = fmaf(g, *cluster.map_shared_rank(sum + h, b), l);
+        }
+        for (int b = 0; b < splits; ++b) share[b * kHeads + h] = l == 0.f ? 0.f : share[b * kHeads + h] / l;
+    }
+    __syncthreads();
+    for (int i = (int)cluster.block_rank() * kThreads + threadIdx.x; i < live_heads * DP; i += splits * kThreads) {
+        const int h = i / DP, x = i % DP;
+        float a = 0.f;
+        for (int b = 0; b < splits; ++b) a = fmaf(share[b * kHeads + h], *cluster.map_shared_rank(&sm_o[0][h][x], b), a);
+        T* out = static_cast<T*>(p.out.ptr) + seq * p.out.token_stride + (head0 + h) * p.out.head_stride;
+        if (x < d) out[x] = from_f<T>(a);
+    }
+    cluster.sync();   // no block leaves while another reads its shared memory
 }
 
-template <typename T, int DP, bool V16>
+template <typename T, int DP, bool FULL>
 cudaError_t launch_one(const CachedAttentionParams& p, int splits, dim3 grid, cudaStream_t stream) {
+    constexpr int join = (kWarps * kHeads * (DP + 2) + (2 + kMaxSplits) * kHeads) * (int)sizeof(float);
+    constexpr int rings = kWarps * Ring<DP, FULL>::kBytes, smem = join > rings ? join : rings;
+    const void* kernel = reinterpret_cast<const void*>(attention_cached_kernel<T, DP, FULL>);
+    cudaError_t e = allow_dynamic_smem(kernel, smem);
+    if (e == cudaSuccess && splits > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = kThreads;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -341,15 +461,15 @@ cudaError_t launch_one(const CachedAttentionParams& p, int splits, dim3 grid, cu
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = splits > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, attention_cached_kernel<T, DP, V16>, p, splits);
+    return cudaLaunchKernelEx(&cfg, attention_cached_kernel<T, DP, FULL>, p, splits);
 }
 
 template <typename T>
 cudaError_t launch_type(const CachedAttentionParams& p, int splits, dim3 grid, cudaStream_t stream) {
     const int d = p.cache.d;
-    if (d <= 32) return launch_one<T, 32, false>(p, splits, grid, stream);
-    if (d <= 64) return d % 16 ? launch_one<T, 64, false>(p, splits, grid, stream) : launch_one<T, 64, true>(p, splits, grid, stream);
-    return d % 16 ? launch_one<T, 128, false>(p, splits, grid, stream) : launch_one<T, 128, true>(p, splits, grid, stream);
+    if (d <= 32) return d == 32 ? launch_one<T, 32, true>(p, splits, grid, stream) : launch_one<T, 32, false>(p, splits, grid, stream);
+    if (d <= 64) return d == 64 ? launch_one<T, 64, true>(p, splits, grid, stream) : launch_one<T, 64, false>(p, splits, grid, stream);
+    return d == 128 ? launch_one<T, 128, true>(p, splits, grid, stream) : launch_one<T, 128, false>(p, splits, grid, stream);
 }
 
 }  // namespace
@@ -358,11 +478,11 @@ cudaError_t launch_attention_cached(const CachedAttentionParams& p, cudaStream_t
     if (p.table.sequences == 0) return cudaSuccess;
     const int group = p.heads / p.cache.kv_heads, parts = (group + kHeads - 1) / kHeads;
     const long long rows = (long long)p.table.sequences * p.cache.kv_heads * parts;
-    // Blocks per sequence and head: enough for three blocks on each SM, as
-    // long as a block keeps 16 tiles of the longest sequence the table holds.
+    // Blocks per sequence and head: enough for three on each SM, as long as a
+    // block keeps 16 tiles of the longest sequence the table holds.
     const long long tiles = (long long)p.table.width * p.cache.page / kTile;
     int splits = 1;
-    while (splits < 8 && rows * splits < 148 * 3 && tiles / (2 * splits) >= 16) splits *= 2;
+    while (splits < kMaxSplits && rows * splits < 148 * 3 && tiles / (2 * splits) >= 16) splits *= 2;
     const dim3 grid((unsigned)(p.table.sequences * (long long)splits), (unsigned)(p.cache.kv_heads * parts));
     return p.dtype == DT_F32 ? launch_type<float>(p, splits, grid, stream)
                              : launch_type<__nv_bfloat16>(p, splits, grid, stream);

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from dataclasses import dataclass
 from typing import List, Optional, Sequence
 
@@ -138,43 +139,16 @@ class _LoadOptions(C.Structure):
                 ("reserved", C.c_int * 4)]
 
 
-class _Tokens(C.Structure):
-    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
-
-
-class _AttentionPackedArgs(C.Structure):
-    _fields_ = [("dtype", C.c_int), ("heads", C.c_int), ("kv_heads", C.c_int), ("d", C.c_int), ("causal", C.c_int),
-                ("scale", C.c_float), ("sequences", C.c_int64), ("total_q", C.c_int64), ("total_k", C.c_int64),
-                ("q", _Tokens), ("k", _Tokens), ("v", _Tokens), ("out", _Tokens), ("q_offsets", C.c_void_p),
-                ("k_offsets", C.c_void_p)]
-
-
-class _PagedCache(C.Structure):
-    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
-                ("pages", C.c_int), ("kv_heads", C.c_int), ("page", C.c_int), ("d", C.c_int)]
-
-
-class _BlockTable(C.Structure):
-    _fields_ = [("pages", C.c_void_p), ("stride", C.c_int64), ("sequences", C.c_int), ("width", C.c_int)]
-
-
-class _CacheTokensArgs(C.Structure):
-    """ppocr_cache_append_args and ppocr_cache_read_args (the last field is `held` / `first`)."""
-    _fields_ = [("dtype", C.c_int), ("total", C.c_int64), ("cache", _PagedCache), ("table", _BlockTable), ("k", _Tokens),
-                ("v", _Tokens), ("offsets", C.c_void_p), ("positions", C.c_void_p)]
-
-
-class _AttentionCachedArgs(C.Structure):
-    _fields_ = [("dtype", C.c_int), ("heads", C.c_int), ("scale", C.c_float), ("cache", _PagedCache),
-                ("table", _BlockTable), ("q", _Tokens), ("out", _Tokens), ("lengths", C.c_void_p)]
-
-
-class _LogitRulesArgs(C.Structure):
-    _fields_ = [("dtype", C.c_int), ("rows", C.c_int), ("vocab", C.c_int), ("states", C.c_int), ("logits", C.c_void_p),
-                ("out", C.c_void_p), ("stride", C.c_int64), ("out_stride", C.c_int64), ("history", C.c_void_p),
-                ("history_offsets", C.c_void_p), ("history_total", C.c_int64), ("repetition", C.c_void_p),
-                ("presence", C.c_void_p), ("frequency", C.c_void_p), ("bias", C.c_void_p), ("mask", C.c_void_p),
-                ("mask_stride", C.c_int64), ("mask_index", C.c_void_p)]
+# The argument structures of the sequence operators in the header's order and the C compiler's layout (every nested
+# structure starts with a pointer and has a size that is a multiple of 8).  Packed as bytes: a ctypes structure per
+# call costs several times the call.
+_TOKENS = "Pqq"
+_CACHE = "PPPPiiii"
+_TABLE = "Pqii"
+_ATTENTION_PACKED = struct.Struct("@iiiiifqqq" + 4 * _TOKENS + "PP").pack
+_CACHE_TOKENS = struct.Struct("@iq" + _CACHE + _TABLE + 2 * _TOKENS + "PP").pack   # append and read
+_ATTENTION_CACHED = struct.Struct("@iif4x" + _CACHE + _TABLE + 2 * _TOKENS + "P").pack
+_LOGIT_RULES = struct.Struct("@iiiiPPqqPPqPPPPPqP").pack
 
 
 _SIZE4 = C.c_size_t * 4
@@ -275,11 +249,11 @@ def library() -> C.CDLL:
         "ppocr_selftest_dispatch": (I, [S, S, C.c_uint32, C.c_uint32, I, I, C.POINTER(C.c_int),
                                         C.POINTER(C.c_int)]),
         "ppocr_gpu_synchronize": (I, [P, P, I]),
-        "ppocr_attention_packed": (I, [P, C.POINTER(_AttentionPackedArgs), P]),
-        "ppocr_cache_append": (I, [P, C.POINTER(_CacheTokensArgs), P]),
-        "ppocr_cache_read": (I, [P, C.POINTER(_CacheTokensArgs), P]),
-        "ppocr_attention_cached": (I, [P, C.POINTER(_AttentionCachedArgs), P]),
-        "ppocr_logit_rules": (I, [P, C.POINTER(_LogitRulesArgs), P]),
+        "ppocr_attention_packed": (I, [P, C.c_char_p, P]),
+        "ppocr_cache_append": (I, [P, C.c_char_p, P]),
+        "ppocr_cache_read": (I, [P, C.c_char_p, P]),
+        "ppocr_attention_cached": (I, [P, C.c_char_p, P]),
+        "ppocr_logit_rules": (I, [P, C.c_char_p, P]),
         "ppocr_recognizer_forward_ctc_rules": (I, [P, FP, S, FP, C.POINTER(C.c_uint32), C.POINTER(C.c_int32), FP, FP]),
     }
     for name, (res, args) in sig.items():
@@ -334,7 +308,8 @@ def inspect_model(path: str, kind: str, size, input_shape: Sequence[int], precis
 class DeviceArray:
     """A device array by its address, shape, element type ("f32", "bf16", "i32", "u32" or "i8"), strides in
     elements (None: contiguous) and device ordinal.  The sequence operators take this or anything that answers
-    as it does: ``data_ptr()``, ``shape``, ``stride()``, ``dtype`` and ``get_device()`` (a torch CUDA tensor)."""
+    as it does: ``data_ptr()``, ``shape``, ``stride()``, ``is_contiguous()``, ``dtype`` and ``get_device()`` (a torch CUDA
+    tensor)."""
 
     def __init__(self, ptr: int, shape: Sequence[int], dtype: str, strides: Optional[Sequence[int]] = None,
                  device: int = 0):
@@ -357,6 +332,14 @@ class DeviceArray:
     def get_device(self) -> int:
         return self._device
 
+    def is_contiguous(self) -> bool:
+        step = 1
+        for n, s in zip(reversed(self.shape), reversed(self._strides)):
+            if n != 1 and s != step:
+                return False
+            step *= n
+        return True
+
 
 @dataclass
 class PagedCache:
@@ -370,14 +353,75 @@ class PagedCache:
 
 _DTYPES = {"f32": "f32", "bf16": "bf16", "i32": "i32", "u32": "i32", "i8": "i8", "torch.float32": "f32",
            "torch.bfloat16": "bf16", "torch.int32": "i32", "torch.uint32": "i32", "torch.int8": "i8"}
-_dtype_names: dict = {}
 
 
-def _dtype_name(dtype) -> str:
-    name = _dtype_names.get(dtype)
-    if name is None:
-        name = _dtype_names[dtype] = _DTYPES.get(str(dtype), str(dtype))
-    return name
+class _DtypeNames(dict):
+    """The name of a framework's element type, looked up by its text once."""
+
+    def __missing__(self, dtype):
+        self[dtype] = name = _DTYPES.get(str(dtype), str(dtype))
+        return name
+
+
+_dtype_names = _DtypeNames()
+_VALUE_TYPES = {"f32": 0, "bf16": 1}
+
+
+def _shape(a, what: str, rank: int):
+    shape = a.shape
+    if len(shape) != rank:
+        raise InvalidInput(f"invalid input: {what} has {len(shape)} axes; expected {rank}")
+    return shape
+
+
+def _value_type(a, what: str):
+    name = _dtype_names[a.dtype]
+    if name not in _VALUE_TYPES:
+        raise InvalidInput(f"invalid input: {what} holds {name}; expected f32 or bf16")
+    return name, _VALUE_TYPES[name]
+
+
+def _refuse(a, what: str, dtype: str, shape, device: int):
+    if len(a.shape) != len(shape):
+        raise InvalidInput(f"invalid input: {what} has {len(a.shape)} axes; expected {len(shape)}")
+    if _dtype_names[a.dtype] != dtype:
+        raise InvalidInput(f"invalid input: {what} holds {_dtype_names[a.dtype]}; expected {dtype}")
+    if tuple(a.shape) != tuple(shape):
+        raise InvalidInput(f"invalid input: {what} has shape {tuple(a.shape)}; expected {tuple(shape)}")
+    if a.get_device() != device:
+        raise InvalidInput(f"invalid input: {what} is on device {a.get_device()}; this handle is on device {device}")
+    raise InvalidInput(f"invalid input: {what} is not contiguous")
+
+
+def _flat(a, what: str, dtype: str, shape, device: int):
+    """Address of a contiguous array of exactly this type and shape (0: absent)."""
+    if a is None:
+        return 0
+    if _dtype_names[a.dtype] != dtype or a.shape != shape or a.get_device() != device or not a.is_contiguous():
+        _refuse(a, what, dtype, shape, device)
+    return a.data_ptr()
+
+
+def _rows(a, what: str, dtype: str, shape, device: int):
+    """Address and strides of an array of exactly this type and shape whose last axis is contiguous."""
+    s = a.stride()
+    if _dtype_names[a.dtype] != dtype or a.shape != shape or a.get_device() != device or (s[-1] != 1 and shape[-1] > 1):
+        _refuse(a, what, dtype, shape, device)
+    return (a.data_ptr(), *s[:-1])
+
+
+def _cuda_stream(stream):
+    if stream is None:
+        return None
+    return getattr(stream, "cuda_stream", stream) or 1   # 1: cudaStreamLegacy
+
+
+def _attention_scale(scale) -> float:
+    if scale is None:
+        return 0.0   # the library's default, d^-1/2
+    if not scale > 0:
+        raise InvalidInput("invalid input: scale must be positive")
+    return scale
 
 
 # ---------------------------------------------------------------------------
@@ -577,105 +621,46 @@ class Gpu:
 
     def synchronize(self, stream=None, timeout_ms: int = 0) -> None:
         """Waits for the stream, then raises what the sequence operators reported (ppocr_gpu_synchronize)."""
-        _check(library().ppocr_gpu_synchronize(self._h, self._stream(stream), int(timeout_ms)))
-
-    @staticmethod
-    def _stream(stream):
-        if stream is None:
-            return None
-        return getattr(stream, "cuda_stream", stream) or 1   # 1: cudaStreamLegacy
-
-    def _array(self, a, what: str, dtype: str, rank: int):
-        """Shape and strides of a device array after the checks that only its owner's framework can answer."""
-        shape = a.shape
-        if len(shape) != rank:
-            raise InvalidInput(f"invalid input: {what} has {len(shape)} axes; expected {rank}")
-        if _dtype_name(a.dtype) != dtype:
-            raise InvalidInput(f"invalid input: {what} holds {_dtype_name(a.dtype)}; expected {dtype}")
-        if a.get_device() != self.device:
-            raise InvalidInput(f"invalid input: {what} is on device {a.get_device()}; this handle is on device {self.device}")
-        return shape, a.stride()
-
-    def _flat(self, a, what: str, dtype: str, shape):
-        """Address of a contiguous array of the given shape (None: absent)."""
-        if a is None:
-            return None
-        got, strides = self._array(a, what, dtype, len(shape))
-        if tuple(got) != tuple(shape):
-            raise InvalidInput(f"invalid input: {what} has shape {tuple(got)}; expected {tuple(shape)}")
-        step = 1
-        for n, s in zip(reversed(got), reversed(strides)):
-            if n > 1 and s != step:
-                raise InvalidInput(f"invalid input: {what} is not contiguous")
-            step *= n
-        return a.data_ptr()
-
-    def _tokens(self, a, what: str, dtype: str, shape):
-        """A [tokens, heads, d] array with a contiguous last axis; -1 in `shape` leaves an extent open."""
-        got, s = self._array(a, what, dtype, 3)
-        if any(w != -1 and g != w for g, w in zip(got, shape)):
-            raise InvalidInput(f"invalid input: {what} has shape {tuple(got)}; expected {tuple(shape)}")
-        if got[2] > 1 and s[2] != 1:
-            raise InvalidInput(f"invalid input: {what}'s last axis is not contiguous")
-        return _Tokens(a.data_ptr(), s[0], s[1])
-
-    @staticmethod
-    def _value_type(a, what: str):
-        name = _dtype_name(a.dtype)
-        if name not in ("f32", "bf16"):
-            raise InvalidInput(f"invalid input: {what} holds {name}; expected f32 or bf16")
-        return name, 0 if name == "f32" else 1
-
-    def _cache(self, cache: PagedCache) -> _PagedCache:
-        pages, heads, page, d = self._array(cache.k, "cache.k", "i8", 4)[0]
-        return _PagedCache(self._flat(cache.k, "cache.k", "i8", (pages, heads, page, d)),
-                           self._flat(cache.v, "cache.v", "i8", (pages, heads, page, d)),
-                           self._flat(cache.k_scales, "cache.k_scales", "f32", (pages, heads)),
-                           self._flat(cache.v_scales, "cache.v_scales", "f32", (pages, heads)), pages, heads, page, d)
-
-    def _table(self, table) -> _BlockTable:
-        (sequences, width), s = self._array(table, "table", "i32", 2)
-        if width > 1 and s[1] != 1:
-            raise InvalidInput("invalid input: table's last axis is not contiguous")
-        return _BlockTable(table.data_ptr(), s[0], sequences, width)
+        _check(library().ppocr_gpu_synchronize(self._h, _cuda_stream(stream), int(timeout_ms)))
 
     def attention_packed(self, q, k, v, q_offsets, k_offsets, out, causal: bool = False, scale: Optional[float] = None,
                          stream=None):
         """softmax(scale q k^T) v per sequence of packed tokens (ppocr_attention_packed): q and out
         [total_q, heads, d], k and v [total_k, kv_heads, d], offsets int32 [sequences + 1]; returns out."""
-        name, dtype = self._value_type(q, "q")
-        total_q, heads, d = self._array(q, "q", name, 3)[0]
-        total_k, kv_heads = self._array(k, "k", name, 3)[0][:2]
-        sequences = self._array(q_offsets, "q_offsets", "i32", 1)[0][0] - 1
-        if sequences < 0:
+        dev = self.device
+        name, dtype = _value_type(q, "q")
+        qs, ks = _shape(q, "q", 3), _shape(k, "k", 3)
+        edges = _shape(q_offsets, "q_offsets", 1)
+        if edges[0] == 0:
             raise InvalidInput("invalid input: q_offsets is empty")
-        args = _AttentionPackedArgs(dtype, heads, kv_heads, d, 1 if causal else 0, self._scale(scale), sequences, total_q,
-                                    total_k, self._tokens(q, "q", name, (total_q, heads, d)),
-                                    self._tokens(k, "k", name, (total_k, kv_heads, d)),
-                                    self._tokens(v, "v", name, (total_k, kv_heads, d)),
-                                    self._tokens(out, "out", name, (total_q, heads, d)),
-                                    self._flat(q_offsets, "q_offsets", "i32", (sequences + 1,)),
-                                    self._flat(k_offsets, "k_offsets", "i32", (sequences + 1,)))
-        _check(library().ppocr_attention_packed(self._h, C.byref(args), self._stream(stream)))
+        ks = (ks[0], ks[1], qs[2])
+        args = _ATTENTION_PACKED(dtype, qs[1], ks[1], qs[2], 1 if causal else 0, _attention_scale(scale), edges[0] - 1,
+                                 qs[0], ks[0], *_rows(q, "q", name, qs, dev), *_rows(k, "k", name, ks, dev),
+                                 *_rows(v, "v", name, ks, dev), *_rows(out, "out", name, qs, dev),
+                                 _flat(q_offsets, "q_offsets", "i32", edges, dev),
+                                 _flat(k_offsets, "k_offsets", "i32", edges, dev))
+        _check(library().ppocr_attention_packed(self._h, args, _cuda_stream(stream)))
         return out
 
-    @staticmethod
-    def _scale(scale) -> float:
-        if scale is None:
-            return 0.0   # the library's default, d^-1/2
-        if not scale > 0:
-            raise InvalidInput("invalid input: scale must be positive")
-        return float(scale)
+    def _paged(self, cache: PagedCache, table):
+        """The cache's and the table's fields, the cache's heads and d, and the table's sequences."""
+        dev, shape = self.device, _shape(cache.k, "cache.k", 4)
+        t = _shape(table, "table", 2)
+        fields = (_flat(cache.k, "cache.k", "i8", shape, dev), _flat(cache.v, "cache.v", "i8", shape, dev),
+                  _flat(cache.k_scales, "cache.k_scales", "f32", shape[:2], dev),
+                  _flat(cache.v_scales, "cache.v_scales", "f32", shape[:2], dev), *shape,
+                  *_rows(table, "table", "i32", t, dev), *t)
+        return fields, shape[1], shape[3], t[0]
 
     def _cache_tokens(self, call, cache, k, v, offsets, positions, what, table, stream):
-        name, dtype = self._value_type(k, "k")
-        c, t = self._cache(cache), self._table(table)
-        total = self._array(k, "k", name, 3)[0][0]
-        args = _CacheTokensArgs(dtype, total, c, t, self._tokens(k, "k", name, (total, c.kv_heads, c.d)),
-                                self._tokens(v, "v", name, (total, c.kv_heads, c.d)),
-                                self._flat(offsets, "offsets", "i32", (t.sequences + 1,)),
-                                self._flat(positions, what, "i32", (t.sequences,)))
-        _check(call(self._h, C.byref(args), self._stream(stream)))
+        dev = self.device
+        name, dtype = _value_type(k, "k")
+        paged, heads, d, sequences = self._paged(cache, table)
+        shape = (_shape(k, "k", 3)[0], heads, d)
+        args = _CACHE_TOKENS(dtype, shape[0], *paged, *_rows(k, "k", name, shape, dev), *_rows(v, "v", name, shape, dev),
+                             _flat(offsets, "offsets", "i32", (sequences + 1,), dev),
+                             _flat(positions, what, "i32", (sequences,), dev))
+        _check(call(self._h, args, _cuda_stream(stream)))
 
     def cache_append(self, cache: PagedCache, k, v, offsets, held, table, stream=None) -> None:
         """Appends packed tokens k and v [total, kv_heads, d] to the sequences' pages (ppocr_cache_append):
@@ -689,14 +674,14 @@ class Gpu:
     def attention_cached(self, cache: PagedCache, q, lengths, table, out, scale: Optional[float] = None, stream=None):
         """Single-token attention over the cache (ppocr_attention_cached): q and out [sequences, heads, d],
         lengths int32 [sequences], table int32 [sequences, width]; returns out."""
-        name, dtype = self._value_type(q, "q")
-        c, t = self._cache(cache), self._table(table)
-        heads = self._array(q, "q", name, 3)[0][1]
-        shape = (t.sequences, heads, c.d)
-        args = _AttentionCachedArgs(dtype, heads, self._scale(scale), c, t, self._tokens(q, "q", name, shape),
-                                    self._tokens(out, "out", name, shape),
-                                    self._flat(lengths, "lengths", "i32", (t.sequences,)))
-        _check(library().ppocr_attention_cached(self._h, C.byref(args), self._stream(stream)))
+        dev = self.device
+        name, dtype = _value_type(q, "q")
+        paged, _, d, sequences = self._paged(cache, table)
+        shape = (sequences, _shape(q, "q", 3)[1], d)
+        args = _ATTENTION_CACHED(dtype, shape[1], _attention_scale(scale), *paged, *_rows(q, "q", name, shape, dev),
+                                 *_rows(out, "out", name, shape, dev),
+                                 _flat(lengths, "lengths", "i32", (sequences,), dev))
+        _check(library().ppocr_attention_cached(self._h, args, _cuda_stream(stream)))
         return out
 
     def logit_rules(self, logits, out, history=None, history_offsets=None, repetition=None, presence=None,
@@ -704,32 +689,28 @@ class Gpu:
         """Penalties over each row's history, class biases and grammar masks (ppocr_logit_rules): logits and out
         [rows, vocab] (out may be logits), history packed int32 ids with offsets [rows + 1], penalties FP32 [rows],
         bias FP32 [vocab], mask int32 words [states, >= ceil(vocab / 32)], mask_index int32 [rows]; returns out."""
-        name, dtype = self._value_type(logits, "logits")
-        (rows, vocab), s = self._array(logits, "logits", name, 2)
-        got, so = self._array(out, "out", name, 2)
-        if tuple(got) != (rows, vocab):
-            raise InvalidInput(f"invalid input: out has shape {tuple(got)}; expected {(rows, vocab)}")
-        if vocab > 1 and (s[1] != 1 or so[1] != 1):
-            raise InvalidInput("invalid input: the last axis of logits or out is not contiguous")
+        dev = self.device
+        name, dtype = _value_type(logits, "logits")
+        shape = _shape(logits, "logits", 2)
+        rows, vocab = shape
         if (history is None) != (history_offsets is None):
             raise InvalidInput("invalid input: history and history_offsets go together")
-        ids = 0 if history is None else self._array(history, "history", "i32", 1)[0][0]
-        states, words, mask_ptr = 0, 0, None
+        ids = (0,) if history is None else _shape(history, "history", 1)
+        states, mask_ptr, words = 0, 0, 0
         if mask is not None:
-            (states, n), sm = self._array(mask, "mask", "i32", 2)
-            if n < -(-vocab // 32) or (n > 1 and sm[1] != 1):
-                raise InvalidInput(f"invalid input: mask rows must be {-(-vocab // 32)} contiguous words or more")
-            words = sm[0] if states > 1 else max(sm[0], n)
-            mask_ptr = mask.data_ptr()
-        args = _LogitRulesArgs(dtype, rows, vocab, states, logits.data_ptr(), out.data_ptr(), s[0], so[0],
-                               self._flat(history, "history", "i32", (ids,)),
-                               self._flat(history_offsets, "history_offsets", "i32", (rows + 1,)), ids,
-                               self._flat(repetition, "repetition", "f32", (rows,)),
-                               self._flat(presence, "presence", "f32", (rows,)),
-                               self._flat(frequency, "frequency", "f32", (rows,)),
-                               self._flat(bias, "bias", "f32", (vocab,)), mask_ptr, words,
-                               self._flat(mask_index, "mask_index", "i32", (rows,)))
-        _check(library().ppocr_logit_rules(self._h, C.byref(args), self._stream(stream)))
+            states, width = m = _shape(mask, "mask", 2)
+            mask_ptr, words = _rows(mask, "mask", "i32", m, dev)
+            if width * 32 < vocab or (states > 1 and words < width):
+                raise InvalidInput(f"invalid input: mask rows must be {-(-vocab // 32)} words or more, apart")
+            words = max(words, width)   # a single row's stride says nothing
+        (x, ld), (y, out_ld) = _rows(logits, "logits", name, shape, dev), _rows(out, "out", name, shape, dev)
+        args = _LOGIT_RULES(dtype, rows, vocab, states, x, y, ld, out_ld, _flat(history, "history", "i32", ids, dev),
+                            _flat(history_offsets, "history_offsets", "i32", (rows + 1,), dev), ids[0],
+                            _flat(repetition, "repetition", "f32", (rows,), dev),
+                            _flat(presence, "presence", "f32", (rows,), dev),
+                            _flat(frequency, "frequency", "f32", (rows,), dev), _flat(bias, "bias", "f32", (vocab,), dev),
+                            mask_ptr, words, _flat(mask_index, "mask_index", "i32", (rows,), dev))
+        _check(library().ppocr_logit_rules(self._h, args, _cuda_stream(stream)))
         return out
 
     def close(self) -> None:
