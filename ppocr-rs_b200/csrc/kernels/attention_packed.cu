@@ -88,7 +88,7 @@ __device__ __forceinline__ void load_tile(T* dst, const T* src, At at, int tile_
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attention_packed_kernel(PackedAttentionParams p, bool vec, bool vec_out) {
+__global__ void __launch_bounds__(kThreads, 3) attention_packed_kernel(PackedAttentionParams p, bool vec, bool vec_out) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int BN = Traits<T>::keys, P = DP + Traits<T>::pad, NT = BN / 8, DT = DP / 8;
     extern __shared__ uint4 smem16[];
@@ -176,6 +176,13 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(PackedAttent
                     mma_bf16_16816(s[n + 1], qf[i], b[2], b[3]);
                 }
         } else {
+            // The tensor cores truncate when they add to an accumulator: the small
+            // cross products are summed apart, the leading ones in chains of two.
+            float rest[NT][4], part[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) rest[n][x] = 0.f;
 #pragma unroll 4
             for (int i = 0; i < DP / 8; ++i) {
                 const float* qa = reinterpret_cast<const float*>(sq) + n0 * P + i * 8 + c;
@@ -190,11 +197,20 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(PackedAttent
                     uint32_t h0, e0, h1, e1;
                     split_tf32(kb[0], h0, e0);
                     split_tf32(kb[4], h1, e1);
-                    mma_tf32_1688(s[n], al, h0, h1);
-                    mma_tf32_1688(s[n], ah, e0, e1);
-                    mma_tf32_1688(s[n], ah, h0, h1);
+                    if (i % 2 == 0) part[n][0] = part[n][1] = part[n][2] = part[n][3] = 0.f;
+                    mma_tf32_1688(rest[n], al, h0, h1);
+                    mma_tf32_1688(rest[n], ah, e0, e1);
+                    mma_tf32_1688(part[n], ah, h0, h1);
+                    if (i % 2 == 1) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) s[n][x] += part[n][x];
+                    }
                 }
             }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) s[n][x] += rest[n][x];
         }
         // Scale, mask, running maximum.
         float t0 = -INFINITY, t1 = -INFINITY;
@@ -251,23 +267,34 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(PackedAttent
         } else {
             // K index c stands for key 2c and c + 4 for key 2c + 1 of the eight,
             // so the scores are the A operand as they are.
+            uint32_t ah[NT][4], al[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                uint32_t ah[4], al[4];
-                split_tf32(s[n][0], ah[0], al[0]);
-                split_tf32(s[n][2], ah[1], al[1]);
-                split_tf32(s[n][1], ah[2], al[2]);
-                split_tf32(s[n][3], ah[3], al[3]);
-                const float* vb = reinterpret_cast<const float*>(vt) + (n * 8 + 2 * c) * P + r;
+                split_tf32(s[n][0], ah[n][0], al[n][0]);
+                split_tf32(s[n][2], ah[n][1], al[n][1]);
+                split_tf32(s[n][1], ah[n][2], al[n][2]);
+                split_tf32(s[n][3], ah[n][3], al[n][3]);
+            }
+            const float* vb = reinterpret_cast<const float*>(vt) + 2 * c * P + r;
 #pragma unroll
-                for (int i = 0; i < DT; ++i) {
+            for (int i = 0; i < DT; ++i) {
+                float rest[4] = {0.f, 0.f, 0.f, 0.f}, part[4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
                     uint32_t h0, e0, h1, e1;
-                    split_tf32(vb[i * 8], h0, e0);
-                    split_tf32(vb[P + i * 8], h1, e1);
-                    mma_tf32_1688(o[i], al, h0, h1);
-                    mma_tf32_1688(o[i], ah, e0, e1);
-                    mma_tf32_1688(o[i], ah, h0, h1);
+                    split_tf32(vb[n * 8 * P + i * 8], h0, e0);
+                    split_tf32(vb[n * 8 * P + P + i * 8], h1, e1);
+                    if (n % 2 == 0) part[0] = part[1] = part[2] = part[3] = 0.f;
+                    mma_tf32_1688(rest, al[n], h0, h1);
+                    mma_tf32_1688(rest, ah[n], e0, e1);
+                    mma_tf32_1688(part, ah[n], h0, h1);
+                    if (n % 2 == 1) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) o[i][x] += part[x];
+                    }
                 }
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[i][x] += rest[x];
             }
         }
         __syncthreads();
@@ -350,6 +377,7 @@ cudaError_t launch_type(const PackedAttentionParams& p, cudaStream_t stream) {
 
 cudaError_t launch_attention_packed(const PackedAttentionParams& p, cudaStream_t stream) {
     if (p.total_q == 0 || p.sequences == 0) return cudaSuccess;
+    if ((long long)p.total_k >= 256ll * p.sequences && attention_tc_supported(p)) return launch_attention_tc(p, stream);
     return p.dtype == DT_F32 ? launch_type<float>(p, stream) : launch_type<__nv_bfloat16>(p, stream);
 }
 

@@ -133,6 +133,41 @@ def test_packed_long(gpu, d, causal, dtype):
     run_packed(gpu, [1100, 3, 900], [1100, 1400, 900], 8, 2, d, dtype, causal, seed=d)
 
 
+@pytest.mark.parametrize("d", [8, 16, 24, 40, 56, 72, 80, 96, 104, 120, 128])
+def test_packed_long_head_sizes(gpu, d):
+    run_packed(gpu, [300, 555, 128], [300, 600, 128], 4, 2, d, "bf16", True, seed=d)
+
+
+@pytest.mark.parametrize("heads,kv", [(1, 1), (3, 1), (10, 2), (7, 7), (40, 1), (128, 1), (129, 1)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_packed_long_groups(gpu, heads, kv, causal):
+    run_packed(gpu, [257, 1, 300], [400, 500, 300], heads, kv, 64, "bf16", causal, seed=heads)
+
+
+@pytest.mark.parametrize("nq,nk", [([1], [256]), ([128, 256], [512, 256]), ([127, 129, 0, 255], [383, 385, 700, 257]),
+                                   ([640, 10, 700], [0, 3, 900]), ([2000], [2000]), ([1, 3, 5], [5000, 300, 1025])])
+@pytest.mark.parametrize("causal", [False, True])
+def test_packed_long_lengths(gpu, nq, nk, causal):
+    for d in (64, 128):
+        run_packed(gpu, nq, nk, 4, 2, d, "bf16", causal, seed=d)
+
+
+def test_packed_growing_scores(gpu):
+    """Keys whose scores grow along the sequence: the running maximum moves again and again."""
+    n, d = 1500, 64
+    for dtype in ("f32", "bf16"):
+        g = rng(21)
+        q, k, v = (torch.randn(n, 2, d, device="cuda", generator=g) for _ in range(3))
+        k = k + q.mean(0, keepdim=True) + torch.arange(n, device="cuda")[:, None, None] / 40 * torch.nn.functional.normalize(q[n // 2:n // 2 + 1], dim=-1)
+        q, k, v = (x.to(DT[dtype]) for x in (q, k, v))
+        out = torch.empty_like(q)
+        s = torch.cuda.current_stream()
+        gpu.attention_packed(q, k, v, offsets([n]), offsets([n]), out, stream=s)
+        gpu.synchronize(s)
+        ref, mag, prod = attend(q.double(), k.double(), v.double(), d ** -0.5)
+        check(out, ref, tolerance(ref, mag, prod, d, n, dtype, 2.0 ** -8 if dtype == "bf16" else 2.0 ** -20), dtype)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("n", [90, 1000])
 def test_packed_strides_and_rows_behind(gpu, dtype, n):
