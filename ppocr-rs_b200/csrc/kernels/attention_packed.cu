@@ -88,7 +88,7 @@ __device__ __forceinline__ void load_tile(T* dst, const T* src, At at, int tile_
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, 3) attention_packed_kernel(PackedAttentionParams p, bool vec, bool vec_out) {
+__global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 5) attention_packed_kernel(PackedAttentionParams p, bool vec, bool vec_out) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int BN = Traits<T>::keys, P = DP + Traits<T>::pad, NT = BN / 8, DT = DP / 8;
     extern __shared__ uint4 smem16[];

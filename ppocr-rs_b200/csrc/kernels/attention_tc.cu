@@ -3,23 +3,20 @@
 //
 // A CTA owns two tiles of 128 rows of one (sequence, KV head); the query heads
 // that share the KV head are rows too (row = token x group + head), so K and V
-// are read once per 256 rows.  Roles (320 threads):
-//   warp 8 / lane 0   TMA: both Q tiles, then K and V tiles of 128 keys into a
+// are read once per 256 rows.  Roles (384 threads):
+//   warp 8            TMA: both Q tiles, then K and V tiles of 128 keys into a
 //                     ring (128-byte swizzled, 64 values of d per row chunk);
-//   warp 9 / lane 0   MMA: S = Q K^T (both operands in shared memory, K-major)
+//   warp 9            MMA: S = Q K^T (both operands in shared memory, K-major)
 //                     into TMEM, and O += P V with P read from TMEM and V
 //                     MN-major as it lies;
 //   warps 0-3, 4-7    softmax of tile 0 and 1, one row per thread: scores from
 //                     TMEM to registers, running maximum and sum, weights back
-//                     as BF16 over the scores' columns.
-// While one tile's softmax runs, the tensor cores work on the other's
+//                     as BF16 over the scores' columns, in two halves so that
+//                     the product of the first runs while the second is made.
+// While one tile's softmax runs, the tensor cores work on the other tile's
 // products.  The maximum that weights are relative to moves only when a score
-// passes it by more than 8 (in log2: weights up to 2^8, exact in BF16's
-// range), so the output accumulator in TMEM is rarely rescaled.
-//
-// Bound: per 128 x 128 tile and d = 128 the products take 1,024 cycles of the
-// tensor cores and the 16,384 exponentials 1,024 cycles of the special
-// function units (16 a cycle).
+// passes it by more than 8 (in log2: weights up to 2^8), so the output
+// accumulator in TMEM is rarely rescaled.
 //
 // Every wait is bounded: on expiry the CTA records a code in status[1], stops,
 // lets its copies and MMAs land, frees its TMEM and returns.  Rows that come
@@ -34,37 +31,68 @@ namespace ppocr {
 
 namespace {
 
-constexpr int kRows = 128, kKeys = 128, kTiles = 2, kThreads = 32 * (4 * kTiles + 2);
-constexpr int kChunk = kKeys * 128;                  // bytes of 128 rows x 64 values
+constexpr int kRows = 128, kKeys = 128, kTiles = 2;
+constexpr int kHalves = 2, kHalf = kKeys / kHalves;          // a tile's weights are handed over in halves
+constexpr int kSoftmaxWarps = 4 * kTiles, kThreads = 32 * kSoftmaxWarps + 128;
+constexpr int kQChunk = kRows * 128, kChunk = kKeys * 128;   // bytes of a tile's rows x 64 values
 constexpr int kTmemCols = 512;
 constexpr float kSlack = 8.f;
+constexpr int kEmulated = 2;   // of every eight pairs of exponentials, on the FMA pipes (0: 263 us, 1: 256, 2: 257, 3: 279)
+
+// 2^x of two values, x <= 2^20, without the special function unit: x = n + f
+// with n the nearest integer (by adding 1.5 x 2^23, whose last mantissa bit is
+// 1), 2^f by the polynomial of degree 4 with the least largest relative error
+// on [-1/2, 1/2] (2.6e-6, a thousandth of the BF16 rounding that follows), and
+// n added to the exponent.  Below 2^-126 it gives about that.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));   // -126; a NaN stays one
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+    const float2 magic = make_float2(12582912.f, 12582912.f);
+    const float2 t = __fadd2_rn(x, magic);
+    const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
+    const float2 f = __fadd2_rn(x, make_float2(-n.x, -n.y));
+    float2 y = __ffma2_rn(f, make_float2(0.0095701f, 0.0095701f), make_float2(0.05591786f, 0.05591786f));
+    y = __ffma2_rn(y, f, make_float2(0.24024745f, 0.24024745f));
+    y = __ffma2_rn(y, f, make_float2(0.69312181f, 0.69312181f));
+    y = __ffma2_rn(y, f, make_float2(0.99999926f, 0.99999926f));
+    return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
+}
 
 template <int DC>   // chunks of 64 values of d
 struct Layout {
-    static constexpr int slots = DC == 1 ? 6 : 4;
-    static constexpr int q_bytes = kTiles * DC * kChunk, slot_bytes = DC * kChunk;
-    static constexpr int smem = q_bytes + slots * slot_bytes + 1024;
+    static constexpr int stages = DC == 1 ? 4 : 2;   // of a V and a K tile each
+    static constexpr int q_bytes = kTiles * DC * kQChunk, tile_bytes = DC * kChunk, stage_bytes = 2 * tile_bytes;
+    static constexpr int smem = q_bytes + stages * stage_bytes + 1024;
 };
 
-// MN-major operand, 128-byte swizzle: rows of 64 values along MN, one per K
-// index; 64-value atoms `atom_stride` bytes apart, groups of 8 K indices 1024.
-__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr, uint32_t atom_stride) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr & 0x3FFFFu) >> 4);
-    d |= (uint64_t)(atom_stride >> 4) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
-}
+// Shared-memory matrix descriptors in two halves: the low one holds the address
+// and the leading byte offset, both in units of 16 bytes, the high one is the
+// same for all tiles (8-row groups 1,024 bytes apart, version 1, 128-byte
+// swizzle).  K-major tiles do not use the leading offset; MN-major ones (rows
+// of 64 values along MN, one per K index) have their 64-value atoms that far
+// apart.
+constexpr uint32_t kDescHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t leading) { return (saddr & 0x3FFFFu) >> 4 | (leading >> 4) << 16; }
 
-// A (BF16, two per column) from TMEM.
-__device__ __forceinline__ void mma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// kind::f16, BF16 operands, FP32 accumulation: both from shared memory, or A
+// (two values per column) from TMEM.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate));
+        "mov.b64 a, {%1, %5};\n\t"
+        "mov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh));
 }
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
@@ -82,6 +110,44 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One lane of a converged warp.  The tcgen05 instructions take their operands
+// from uniform registers: under elect.sync the compiler knows that one lane
+// runs them, under `lane == 0` it loops over the lanes that might (an MMA then
+// took 120 cycles to issue, 64 to execute).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(one));
+    return one;
+}
+
+// tc::mbar_wait without its first read of the global timer, which takes longer
+// than most waits here: the timer is read once in 4,096 tries.
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, const volatile int* abort) {
+    const uint32_t addr = tc::smem_u32(bar);
+    uint64_t start = 0;
+    for (uint32_t i = 1;; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}\n"
+            : "=r"(done)
+            : "r"(addr), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if ((i & 63) == 0 && *abort) return false;
+        if ((i & 4095) == 0) {
+            const uint64_t now = tc::globaltimer_ns();
+            if (start == 0) start = now;
+            else if (now - start > tc::kWaitNs) return false;
+        }
+    }
+}
 
 // The work of one CTA, from its id.
 struct Work {
@@ -126,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                                                                    PackedAttentionParams p, bool vec_out) {
     using L = Layout<DC>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t q_full, full[L::slots], empty[L::slots], s_full[kTiles], p_full[kTiles], o_full[kTiles], drain;
+    __shared__ __align__(8) uint64_t q_full, full[L::stages], empty[L::stages], s_full[kTiles], p_full[kTiles][kHalves], o_full[kTiles], drain;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
     Work w;
@@ -140,20 +206,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
 
     if (threadIdx.x == 0) {
         tc::mbar_init(&q_full, 1);
-        for (int i = 0; i < L::slots; ++i) {
+        for (int i = 0; i < L::stages; ++i) {
             tc::mbar_init(&full[i], 1);
             tc::mbar_init(&empty[i], 1);
         }
         for (int t = 0; t < kTiles; ++t) {
             tc::mbar_init(&s_full[t], 1);
-            tc::mbar_init(&p_full[t], 128);
+            for (int h = 0; h < kHalves; ++h) tc::mbar_init(&p_full[t][h], 128);
             tc::mbar_init(&o_full[t], 1);
         }
         tc::mbar_init(&drain, 1);
         abort_flag = 0;
         tc::mbar_fence_init();
     }
-    if (warp == 4 * kTiles) tc::tmem_alloc(&tmem_slot, kTmemCols);
+    if (warp == kSoftmaxWarps) tc::tmem_alloc(&tmem_slot, kTmemCols);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -164,93 +230,120 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         abort_flag = 1;
     };
 
-    if (warp == 4 * kTiles) {
-        if (lane == 0 && steps > 0) {
+    // Stage 0 of the ring holds K of step 0, stage j + 1 V of step j and K of step
+    // j + 1 (which the last stage lacks).
+    // The softmax warpgroups take the registers that the copying and issuing one
+    // leaves: 2 x 208 + 88 of the 3 x 168 that the block is launched with.
+    if (warp >= kSoftmaxWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == kSoftmaxWarps && steps > 0) {
             int q_tiles = 0;
             for (int t = 0; t < kTiles; ++t) q_tiles += w.rows[t] > 0;
-            // A Q box is per x group rows; rows past the tensor are zeros.
-            tc::mbar_expect_tx(&q_full, (uint32_t)(q_tiles * DC * w.per * w.group * 128));
-            for (int t = 0; t < q_tiles; ++t)
-                for (int c = 0; c < DC; ++c)
-                    tma_load_3d(sq + (t * DC + c) * kChunk, &map_q, &q_full, c * 64, w.kv * w.group, w.qs.begin + w.token0 + t * w.per);
-            // Tile i of the ring: K of step i / 2, then V of it.
+            if (elect_one()) {
+                // A Q box is per x group rows; rows past the tensor are zeros.
+                tc::mbar_expect_tx(&q_full, (uint32_t)(q_tiles * DC * w.per * w.group * 128));
+                for (int t = 0; t < q_tiles; ++t)
+                    for (int c = 0; c < DC; ++c)
+                        tma_load_3d(sq + (t * DC + c) * kQChunk, &map_q, &q_full, c * 64, w.kv * w.group, w.qs.begin + w.token0 + t * w.per);
+            }
             int i = 0;
-            for (; i < 2 * steps; ++i) {
-                const int s = i % L::slots;
-                if (i >= L::slots && !tc::mbar_wait(&empty[s], (i / L::slots + 1) & 1, false, tc::kWaitNs, &abort_flag)) {
+            for (; i <= steps; ++i) {
+                const int s = i % L::stages;
+                if (i >= L::stages && !__all_sync(0xffffffffu, wait_phase(&empty[s], (i / L::stages + 1) & 1, &abort_flag))) {
                     expired(1);
                     break;
                 }
-                tc::mbar_expect_tx(&full[s], (uint32_t)L::slot_bytes);
-                for (int c = 0; c < DC; ++c)
-                    tma_load_3d(ring + s * L::slot_bytes + c * kChunk, i & 1 ? &map_v : &map_k, &full[s], c * 64, w.kv,
-                                w.ks.begin + (i >> 1) * kKeys);
+                if (elect_one()) {
+                    tc::mbar_expect_tx(&full[s], (uint32_t)(i == 0 || i == steps ? L::tile_bytes : L::stage_bytes));
+                    uint8_t* to = ring + s * L::stage_bytes;
+                    for (int c = 0; i < steps && c < DC; ++c)
+                        tma_load_3d(to + L::tile_bytes + c * kChunk, &map_k, &full[s], c * 64, w.kv, w.ks.begin + i * kKeys);
+                    for (int c = 0; i > 0 && c < DC; ++c)
+                        tma_load_3d(to + c * kChunk, &map_v, &full[s], c * 64, w.kv, w.ks.begin + (i - 1) * kKeys);
+                }
+                __syncwarp();
             }
             // No copy is in flight when the CTA ends, however it ends.
             tc::mbar_wait(&q_full, 0, false);
-            for (int b = max(0, i - L::slots); b < i; ++b) tc::mbar_wait(&full[b % L::slots], (b / L::slots) & 1, false);
-        }
-    } else if (warp == 4 * kTiles + 1) {
-        if (lane == 0 && steps > 0) {
-            const int k_steps = (p.d + 15) / 16, n_out = k_steps * 16;
+            for (int b = max(0, i - L::stages); b < i; ++b) tc::mbar_wait(&full[b % L::stages], (b / L::stages) & 1, false);
+        } else if (warp == kSoftmaxWarps + 1 && steps > 0) {
+            // An issued instruction costs this warp 30 to 50 cycles and a wait 200
+            // although its phase is long complete, so there are as few as can be:
+            // all 4 DC steps over d (past d both operands are zeros), one commit
+            // per tile and step, one to release a stage, and barriers that are
+            // waited for together on different lanes.
+            const int n_out = (p.d + 15) / 16 * 16;
             const uint32_t id_s = tc::idesc_bf16(kRows, kKeys);
             const uint32_t id_o = tc::idesc_bf16(kRows, n_out) | (1u << 16);   // B MN-major
+            const uint32_t q_desc = desc_low(tc::smem_u32(sq), 0), k_desc = desc_low(tc::smem_u32(ring) + L::tile_bytes, 0);
+            const uint32_t v_desc = desc_low(tc::smem_u32(ring), kChunk);
             bool ok = true;
             auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-                if (ok && !tc::mbar_wait(bar, parity, false, tc::kWaitNs, &abort_flag)) {
+                if (ok && !__all_sync(0xffffffffu, wait_phase(bar, parity, &abort_flag))) {
                     expired(code);
                     ok = false;
                 }
-                if (ok) tc::fence_after();
+                tc::fence_after();
             };
-            auto scores = [&](int t, int j) {
-                const uint32_t q = tc::smem_u32(sq + t * DC * kChunk), k = tc::smem_u32(ring + (2 * j % L::slots) * L::slot_bytes);
-                for (int x = 0; x < k_steps; ++x) {
-                    const uint32_t at = (x >> 2) * kChunk + (x & 3) * 32;
-                    tc::mma_bf16(tm_s[t], tc::sw128_desc(q + at), tc::sw128_desc(k + at), id_s, x > 0);
-                }
+            // One lane: the scores of tile t from the K tile at `k`.
+            auto scores = [&](int t, uint32_t k) {
+#pragma unroll
+                for (int x = 0; x < 4 * DC; ++x)
+                    mma_ss(tm_s[t], q_desc + (((t * DC + (x >> 2)) * kQChunk + (x & 3) * 32) >> 4),
+                           k + (((x >> 2) * kChunk + (x & 3) * 32) >> 4), id_s, x > 0);
                 tc::commit(&s_full[t]);
             };
-            wait(&q_full, 0, 2);
-            wait(&full[0], 0, 3);
-            if (ok) {
+            wait(lane ? &full[0] : &q_full, 0, 2);
+            if (ok && elect_one()) {
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t)
-                    if (n[t] > 0) scores(t, 0);
+                    if (n[t] > 0) scores(t, k_desc);
                 tc::commit(&empty[0]);
             }
+            __syncwarp();
+            int s = 1, phase = 0;
             for (int j = 0; j < steps && ok; ++j) {
-                const int v_at = 2 * j + 1, k_at = 2 * j + 2;
+                // The stage, and tile 0's first weights.
+                const bool own = lane && j < n[0];
+                wait(own ? &p_full[0][0] : &full[s], own ? j & 1 : phase, 3);
+                const uint32_t v = v_desc + s * (L::stage_bytes >> 4), k = k_desc + s * (L::stage_bytes >> 4);
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t) {
-                    if (!ok) break;
-                    if (j < n[t]) {
-                        wait(&p_full[t], j & 1, 4);
-                        wait(&full[v_at % L::slots], (v_at / L::slots) & 1, 5);
-                        if (!ok) break;
-                        const uint32_t v = tc::smem_u32(ring + (v_at % L::slots) * L::slot_bytes);
 #pragma unroll
-                        for (int x = 0; x < kKeys / 16; ++x)
-                            mma_bf16_ts(tm_o[t], tm_s[t] + x * 8, sw128_desc_mn(v + x * 2048, kChunk), id_o, (j | x) > 0);
-                        if (j + 1 == n[t]) tc::commit(&o_full[t]);
-                    }
-                    if (t == kTiles - 1) tc::commit(&empty[v_at % L::slots]);
-                    // The MMAs run in order: these scores overwrite the weights that
-                    // the product above has read by then, and their commit covers it.
-                    if (j + 1 < n[t]) {
-                        wait(&full[k_at % L::slots], (k_at / L::slots) & 1, 6);
+                    for (int h = 0; h < kHalves; ++h) {
+                        if (t + h > 0 && j < n[t]) wait(&p_full[t][h], j & 1, 4);
                         if (!ok) break;
-                        scores(t, j + 1);
+                        if (elect_one()) {
+                            if (j < n[t]) {
+#pragma unroll
+                                for (int x = h * kHalf / 16; x < (h + 1) * kHalf / 16; ++x)
+                                    mma_ts(tm_o[t], tm_s[t] + x * 8, v + x * (2048 >> 4), id_o, (j | x) > 0);
+                                // The MMAs run in order: the next scores overwrite the weights
+                                // that the product has read by then, and their commit covers it.
+                                if (h + 1 == kHalves) {
+                                    if (j + 1 < n[t]) scores(t, k);
+                                    else tc::commit(&o_full[t]);
+                                }
+                            }
+                            if (t + 1 == kTiles && h + 1 == kHalves) tc::commit(&empty[s]);
+                        }
+                        __syncwarp();
                     }
                 }
-                if (ok && j + 1 < steps) tc::commit(&empty[k_at % L::slots]);
+                if (++s == L::stages) {
+                    s = 0;
+                    phase ^= 1;
+                }
             }
-            // Every MMA this thread issued completes before TMEM is freed.
-            tc::commit(&drain);
+            // Every MMA this warp issued completes before TMEM is freed.
+            if (elect_one()) tc::commit(&drain);
+            __syncwarp();
             tc::mbar_wait(&drain, 0, false);
         }
     } else {
-        const int t = warp >> 2, row = (warp & 3) * 32 + lane, live = t ? w.rows[1] : w.rows[0], tiles = t ? n[1] : n[0];
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+        const int live = t ? w.rows[1] : w.rows[0], tiles = t ? n[1] : n[0];
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = (t ? tm_s[1] : tm_s[0]) + lanes, to = (t ? tm_o[1] : tm_o[0]) + lanes;
         const int n_out = (p.d + 15) / 16 * 16;
@@ -259,29 +352,41 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         const int sure = (int)__reduce_min_sync(0xffffffffu, (unsigned)keys);
         float top = -INFINITY, ref = 0.f, sum = 0.f;   // ref: top, 0 while it is -infinity
         bool ok = true;
-        for (int j = 0; j < tiles; ++j) {
-            ok = __all_sync(0xffffffffu, tc::mbar_wait(&s_full[t], j & 1, false, tc::kWaitNs, &abort_flag));
-            if (!ok) {
-                if (lane == 0) expired(7);
-                break;
-            }
+        auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+            ok = __all_sync(0xffffffffu, wait_phase(bar, parity, &abort_flag));
+            if (!ok) expired(code);
             tc::fence_after();
+        };
+        for (int j = 0; j < tiles; ++j) {
+            wait(&s_full[t], j & 1, 5);
+            if (!ok) break;
             uint32_t r[kKeys];
-#pragma unroll
-            for (int c = 0; c < kKeys; c += 16) tc::tmem_ld16_async(ts + c, r + c);
-            tc::tmem_wait_ld_regs(r);
             float* s = reinterpret_cast<float*>(r);
-            if ((j + 1) * kKeys > sure) {
-                const int left = keys - j * kKeys;
+            // Each quarter's maximum while the next quarter is on its way.
+            constexpr int Q = kKeys / 4;
+            float m[4];
+            auto load = [&](int c0) {
 #pragma unroll
-                for (int c = 0; c < kKeys; ++c)
-                    if (c >= left) s[c] = -INFINITY;
+                for (int c = c0; c < c0 + Q; c += 16) tc::tmem_ld16_async(ts + c, r + c);
+            };
+            load(0);
+#pragma unroll
+            for (int c0 = 0; c0 < kKeys; c0 += Q) {
+                tc::tmem_wait_ld();
+#pragma unroll
+                for (int c = c0; c < c0 + Q; ++c) asm volatile("" : "+r"(r[c]));
+                if (c0 + Q < kKeys) load(c0 + Q);
+                if ((j + 1) * kKeys > sure) {
+                    const int left = keys - j * kKeys;
+#pragma unroll
+                    for (int c = c0; c < c0 + Q; ++c)
+                        if (c >= left) s[c] = -INFINITY;
+                }
+#pragma unroll
+                for (int c = c0; c < c0 + Q; c += 4)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) m[i] = c == 0 ? s[c + i] : fmaxf(m[i], s[c + i]);
             }
-            float m[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-            for (int c = 4; c < kKeys; c += 4)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) m[i] = fmaxf(m[i], s[c + i]);
             const float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * scale;
             if (__any_sync(0xffffffffu, most > top + kSlack)) {
                 const float next = fmaxf(top, most);
@@ -304,25 +409,24 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
 #pragma unroll
             for (int c = 0; c < kKeys; c += 2) {
                 float2 x = __ffma2_rn(make_float2(s[c], s[c + 1]), a, b);
-                x = make_float2(exp2_hw(x.x), exp2_hw(x.y));
+                x = c / 2 % 8 < kEmulated ? exp2_fma(x) : make_float2(exp2_hw(x.x), exp2_hw(x.y));
                 part[(c >> 1) & 1] = __fadd2_rn(part[(c >> 1) & 1], x);
-                const __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
-                r[c / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                const __nv_bfloat162 v = __floats2bfloat162_rn(x.x, x.y);
+                r[c / 2] = *reinterpret_cast<const uint32_t*>(&v);
+                if (c % 32 == 30) tmem_st16(ts + c / 32 * 16, r + c / 32 * 16);
+                if ((c + 2) % kHalf == 0) {
+                    tmem_wait_st();
+                    tc::fence_before();
+                    tc::mbar_arrive(&p_full[t][c / kHalf]);
+                }
             }
             sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
-#pragma unroll
-            for (int c = 0; c < kKeys / 2; c += 16) tmem_st16(ts + c, r + c);
-            tmem_wait_st();
-            tc::fence_before();
-            tc::mbar_arrive(&p_full[t]);
         }
-        if (ok && tiles > 0) {
-            ok = __all_sync(0xffffffffu, tc::mbar_wait(&o_full[t], 0, false, tc::kWaitNs, &abort_flag));
-            if (!ok && lane == 0) expired(8);
-            tc::fence_after();
-        }
+        if (ok && tiles > 0) wait(&o_full[t], 0, 6);
         if (ok && live) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            // top: -infinity where every score is (or is no number), and then the
+            // emulated weights are not quite 0.
+            const float inv = sum == 0.f || (top == -INFINITY && !isnan(sum)) ? 0.f : 1.f / sum;
             const int token = w.token0 + t * w.per + row / w.group, head = w.kv * w.group + row % w.group;
             __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out.ptr) + (w.qs.begin + (long long)token) * p.out.token_stride +
                                  head * p.out.head_stride;
@@ -352,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(p.k.ptr) + (long long)w.ks.begin * p.k.token_stride + w.kv * p.k.head_stride;
             const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(p.v.ptr) + (long long)w.ks.begin * p.v.token_stride + w.kv * p.v.head_stride;
             for (unsigned again = __ballot_sync(0xffffffffu, bad); again; again &= again - 1) {
-                const int l = __ffs(again) - 1, rr = (warp & 3) * 32 + l;
+                const int rr = (warp & 3) * 32 + __ffs(again) - 1;
                 const int tk = w.qs.begin + w.token0 + t * w.per + rr / w.group, hd = w.kv * w.group + rr % w.group;
                 __syncwarp();
                 attend_row<__nv_bfloat16>(q + tk * p.q.token_stride + hd * p.q.head_stride, k, p.k.token_stride, v, p.v.token_stride,
@@ -363,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     }
     tc::fence_before();
     __syncthreads();
-    if (warp == 4 * kTiles) {
+    if (warp == kSoftmaxWarps) {
         tc::fence_after();
         tc::tmem_dealloc(tmem, kTmemCols);
     }
