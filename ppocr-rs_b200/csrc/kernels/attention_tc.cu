@@ -168,18 +168,20 @@ __device__ __forceinline__ bool find_work(const PackedAttentionParams& p, Work& 
     w.per = kRows / w.group;
     w.kv = blockIdx.x % p.kv_heads;
     const int step = kTiles * w.per;   // queries of a CTA
-    const long long pieces = gridDim.x / p.kv_heads, at = blockIdx.x / p.kv_heads;
-    const long long id = p.causal ? pieces - 1 - at : at;   // the longest rows first
-    auto first_id = [&](int i) { return (long long)seq_offset(p.q_offsets, p.uniform, i, p.total_q) / step + i; };
+    const int pieces = gridDim.x / p.kv_heads, at = blockIdx.x / p.kv_heads;
+    const int id = p.causal ? pieces - 1 - at : at;   // the longest rows first
+    auto first_id = [&](int i) { return seq_offset(p.q_offsets, p.uniform, i, p.total_q) / step + i; };
     w.seq = find_owner(p.sequences, id, first_id);
     w.qs = seq_span(p.q_offsets, p.uniform, w.seq, p.total_q, p.status);
     w.ks = seq_span(p.k_offsets, p.uniform, w.seq, p.total_k, p.status);
-    const long long first = (id - first_id(w.seq)) * step;
-    if (first < 0 || first >= w.qs.len) return false;
-    w.token0 = (int)first;
+    const int index = id - first_id(w.seq);
+    if (index < 0 || index > w.qs.len / step) return false;
+    w.token0 = index * step;
+    const int left = w.qs.len - w.token0;
+    if (left <= 0) return false;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
-        w.rows[t] = min(max(w.qs.len - w.token0 - t * w.per, 0), w.per) * w.group;
+        w.rows[t] = (left >= (t + 1) * w.per ? w.per : left > t * w.per ? left - t * w.per : 0) * w.group;
         w.keys[t] = w.rows[t] ? keys_of(p, w, t, w.rows[t] - 1) : 0;
     }
     return true;
@@ -204,7 +206,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     const int n[kTiles] = {(w.keys[0] + kKeys - 1) / kKeys, (w.keys[1] + kKeys - 1) / kKeys};
     const int steps = max(n[0], n[1]);
 
-    if (threadIdx.x == 0) {
+    // Stage 0 of the ring holds K of step 0, stage j + 1 V of step j and K of step
+    // j + 1 (which the last stage lacks).  One lane of the copying warp.
+    auto load_stage = [&](int i) {
+        const int s = i % L::stages;
+        tc::mbar_expect_tx(&full[s], (uint32_t)(i == 0 || i == steps ? L::tile_bytes : L::stage_bytes));
+        uint8_t* to = ring + s * L::stage_bytes;
+        for (int c = 0; i < steps && c < DC; ++c)
+            tma_load_3d(to + L::tile_bytes + c * kChunk, &map_k, &full[s], c * 64, w.kv, w.ks.begin + i * kKeys);
+        for (int c = 0; i > 0 && c < DC; ++c)
+            tma_load_3d(to + c * kChunk, &map_v, &full[s], c * 64, w.kv, w.ks.begin + (i - 1) * kKeys);
+    };
+    if (warp == kSoftmaxWarps && elect_one()) {
         tc::mbar_init(&q_full, 1);
         for (int i = 0; i < L::stages; ++i) {
             tc::mbar_init(&full[i], 1);
@@ -218,8 +231,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         tc::mbar_init(&drain, 1);
         abort_flag = 0;
         tc::mbar_fence_init();
+        if (steps > 0) {
+            // The first copies start while the others set up.  A Q box is per x
+            // group rows; rows past the tensor are zeros.
+            const int q_tiles = 1 + (w.rows[1] > 0);
+            tc::mbar_expect_tx(&q_full, (uint32_t)(q_tiles * DC * w.per * w.group * 128));
+            for (int t = 0; t < q_tiles; ++t)
+                for (int c = 0; c < DC; ++c)
+                    tma_load_3d(sq + (t * DC + c) * kQChunk, &map_q, &q_full, c * 64, w.kv * w.group, w.qs.begin + w.token0 + t * w.per);
+            load_stage(0);
+        }
     }
-    if (warp == kSoftmaxWarps) tc::tmem_alloc(&tmem_slot, kTmemCols);
+    if (warp == kSoftmaxWarps + 1) tc::tmem_alloc(&tmem_slot, kTmemCols);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -230,37 +253,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         abort_flag = 1;
     };
 
-    // Stage 0 of the ring holds K of step 0, stage j + 1 V of step j and K of step
-    // j + 1 (which the last stage lacks).
     // The softmax warpgroups take the registers that the copying and issuing one
     // leaves: 2 x 208 + 88 of the 3 x 168 that the block is launched with.
     if (warp >= kSoftmaxWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == kSoftmaxWarps && steps > 0) {
-            int q_tiles = 0;
-            for (int t = 0; t < kTiles; ++t) q_tiles += w.rows[t] > 0;
-            if (elect_one()) {
-                // A Q box is per x group rows; rows past the tensor are zeros.
-                tc::mbar_expect_tx(&q_full, (uint32_t)(q_tiles * DC * w.per * w.group * 128));
-                for (int t = 0; t < q_tiles; ++t)
-                    for (int c = 0; c < DC; ++c)
-                        tma_load_3d(sq + (t * DC + c) * kQChunk, &map_q, &q_full, c * 64, w.kv * w.group, w.qs.begin + w.token0 + t * w.per);
-            }
-            int i = 0;
+            int i = 1;
             for (; i <= steps; ++i) {
-                const int s = i % L::stages;
-                if (i >= L::stages && !__all_sync(0xffffffffu, wait_phase(&empty[s], (i / L::stages + 1) & 1, &abort_flag))) {
+                if (i >= L::stages && !__all_sync(0xffffffffu, wait_phase(&empty[i % L::stages], (i / L::stages + 1) & 1, &abort_flag))) {
                     expired(1);
                     break;
                 }
-                if (elect_one()) {
-                    tc::mbar_expect_tx(&full[s], (uint32_t)(i == 0 || i == steps ? L::tile_bytes : L::stage_bytes));
-                    uint8_t* to = ring + s * L::stage_bytes;
-                    for (int c = 0; i < steps && c < DC; ++c)
-                        tma_load_3d(to + L::tile_bytes + c * kChunk, &map_k, &full[s], c * 64, w.kv, w.ks.begin + i * kKeys);
-                    for (int c = 0; i > 0 && c < DC; ++c)
-                        tma_load_3d(to + c * kChunk, &map_v, &full[s], c * 64, w.kv, w.ks.begin + (i - 1) * kKeys);
-                }
+                if (elect_one()) load_stage(i);
                 __syncwarp();
             }
             // No copy is in flight when the CTA ends, however it ends.
@@ -422,20 +426,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             }
             sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
         }
-        if (ok && tiles > 0) wait(&o_full[t], 0, 6);
+        // A tile without keys still waits for its Q, whose place its output takes.
+        if (ok && live && steps > 0) wait(tiles > 0 ? &o_full[t] : &q_full, 0, 6);
         if (ok && live) {
             // top: -infinity where every score is (or is no number), and then the
             // emulated weights are not quite 0.
             const float inv = sum == 0.f || (top == -INFINITY && !isnan(sum)) ? 0.f : 1.f / sum;
-            const int token = w.token0 + t * w.per + row / w.group, head = w.kv * w.group + row % w.group;
-            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out.ptr) + (w.qs.begin + (long long)token) * p.out.token_stride +
-                                 head * p.out.head_stride;
+            // Rows leave through shared memory (over the tile's Q, which the last
+            // scores have read), 16 bytes a lane along the row: stored as they lie
+            // in TMEM, a row per lane, they took 3,000 cycles.
+            uint8_t* stage = sq + t * DC * kQChunk;
+            auto piece = [&](int r, int x) { return stage + (x >> 3) * kQChunk + r * 128 + (((x & 7) ^ (r & 7)) << 4); };
             bool bad = false;
+#pragma unroll 2
             for (int c = 0; c < n_out; c += 16) {
-                uint32_t o[16] = {};
+                uint32_t o[16] = {}, h[8];
                 if (tiles > 0) tc::tmem_ld16(to + c, o);
-                if (row >= live) continue;
-                uint32_t h[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float x = __uint_as_float(o[2 * i]) * inv, y = __uint_as_float(o[2 * i + 1]) * inv;
@@ -443,13 +449,25 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                     const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
                     h[i] = *reinterpret_cast<const uint32_t*>(&v);
                 }
-                if (vec_out) {   // d is a multiple of 8
-                    *reinterpret_cast<uint4*>(out + c) = make_uint4(h[0], h[1], h[2], h[3]);
-                    if (c + 8 < p.d) *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(h[4], h[5], h[6], h[7]);
+                *reinterpret_cast<uint4*>(piece(row, c / 8)) = make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4*>(piece(row, c / 8 + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+            }
+            bad &= row < live;
+            __syncwarp();
+            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out.ptr) + (long long)(w.qs.begin + w.token0 + t * w.per) * p.out.token_stride +
+                                 (long long)w.kv * w.group * p.out.head_stride;
+            const long long mine = (row / w.group) * p.out.token_stride + (row % w.group) * p.out.head_stride;
+            const int width = p.d / 8, shift = width > 8 ? 4 : width > 4 ? 3 : width > 2 ? 2 : width - 1;   // 2^shift lanes a row
+            for (int l0 = 0; l0 < 32; l0 += 32 >> shift) {
+                const int l = l0 + (lane >> shift), r = (warp & 3) * 32 + l, x = lane & ((1 << shift) - 1);
+                const long long off = __shfl_sync(0xffffffffu, mine, l);
+                if (r >= live || x >= width) continue;
+                const uint4 v = *reinterpret_cast<const uint4*>(piece(r, x));
+                if (vec_out) {
+                    *reinterpret_cast<uint4*>(out + off + x * 8) = v;
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (c + i < p.d) out[c + i] = reinterpret_cast<const __nv_bfloat16*>(h)[i];
+                    for (int i = 0; i < 8; ++i) out[off + x * 8 + i] = reinterpret_cast<const __nv_bfloat16*>(&v)[i];
                 }
             }
             const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q.ptr);
@@ -467,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     }
     tc::fence_before();
     __syncthreads();
-    if (warp == kSoftmaxWarps) {
+    if (warp == kSoftmaxWarps + 1) {
         tc::fence_after();
         tc::tmem_dealloc(tmem, kTmemCols);
     }

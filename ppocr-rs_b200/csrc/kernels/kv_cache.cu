@@ -88,9 +88,10 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(CacheAppendParam
     __shared__ uint32_t top[kThreads / 32];
     // A sequence's n new tokens touch at most n / page + 2 pages.
     const int page = p.cache.page, d8 = p.cache.d / 8, head = blockIdx.y;
-    auto first_id = [&](int i) { return (long long)seq_offset(p.offsets, 0, i, p.total) / page + 2ll * i; };
-    const int seq = find_owner(p.table.sequences, blockIdx.x, first_id);
-    const int index = (int)(blockIdx.x - first_id(seq));   // of the pages this sequence's new tokens touch
+    const int page_shift = 31 - __clz(page), id = blockIdx.x;
+    auto first_id = [&](int i) { return (seq_offset(p.offsets, 0, i, p.total) >> page_shift) + 2 * i; };
+    const int seq = find_owner(p.table.sequences, id, first_id);
+    const int index = id - first_id(seq);   // of the pages this sequence's new tokens touch
     const Span span = seq_span(p.offsets, 0, seq, p.total, p.status);
     const int held = p.held[seq];
     if (span.len == 0 || index < 0) return;

@@ -27,14 +27,19 @@ __device__ __forceinline__ Span seq_span(const int32_t* offsets, int uniform, in
 
 // Deals ids to the sequences without a prefix sum: sequence i owns the ids
 // [first(i), first(i + 1)), where first() needs i's offset alone and grows with
-// i by at least i's number of pieces (some ids then own no piece).  The owner
-// of `id` is found by bisection; every thread gets the answer.
-template <typename First>
-__device__ __forceinline__ int find_owner(int sequences, long long id, First first) {
-    int lo = 0, hi = sequences;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (first(mid) <= id) lo = mid; else hi = mid;
+// i by at least i's number of pieces (some ids then own no piece).  A converged
+// warp finds the owner of `id`, 32 sequences a round: one round trip to memory
+// for up to 32 sequences, two for 1,024.
+template <typename Id, typename First>
+__device__ __forceinline__ int find_owner(int sequences, Id id, First first) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, n = sequences;   // the owner is one of [lo, lo + n)
+    while (n > 1) {
+        const int step = (n + 31) / 32, at = lane * step;
+        const unsigned mask = __ballot_sync(0xffffffffu, at < n && first(lo + at) <= id) | 1u;
+        const int skip = (31 - __clz(mask)) * step;
+        lo += skip;
+        n = min(step, n - skip);
     }
     return lo;
 }

@@ -86,15 +86,19 @@ def packed_reference(q, k, v, nq, nk, causal, scale, dtype):
 
 def run_packed(gpu, nq, nk, heads, kv, d, dtype, causal, scale=None, seed=0, stream=None):
     g = rng(seed)
-    q = torch.randn(sum(nq), heads, d, device="cuda", generator=g).to(DT[dtype])
-    k = torch.randn(sum(nk), kv, d, device="cuda", generator=g).to(DT[dtype])
-    v = torch.randn(sum(nk), kv, d, device="cuda", generator=g).to(DT[dtype])
+    behind = 150   # tokens behind the last sequence: no number among the inputs, left as they were in the output
+    q = torch.randn(sum(nq) + behind, heads, d, device="cuda", generator=g).to(DT[dtype])
+    k = torch.randn(sum(nk) + behind, kv, d, device="cuda", generator=g).to(DT[dtype])
+    v = torch.randn(sum(nk) + behind, kv, d, device="cuda", generator=g).to(DT[dtype])
+    for x in (q, k, v):
+        x[-behind:] = math.nan
     out = torch.full_like(q, 7.0)
     gpu.attention_packed(q, k, v, offsets(nq), offsets(nk), out, causal=causal, scale=scale,
                          stream=torch.cuda.current_stream())
     gpu.synchronize(torch.cuda.current_stream())
     ref, tol = packed_reference(q, k, v, nq, nk, causal, d ** -0.5 if scale is None else scale, dtype)
-    check(out, ref, tol, f"{nq} {nk} {heads}/{kv} d{d} {dtype} causal={causal}")
+    assert (out[sum(nq):] == 7.0).all()
+    check(out[:sum(nq)], ref, tol, f"{nq} {nk} {heads}/{kv} d{d} {dtype} causal={causal}")
 
 
 LENGTHS = [
@@ -145,7 +149,8 @@ def test_packed_long_groups(gpu, heads, kv, causal):
 
 
 @pytest.mark.parametrize("nq,nk", [([1], [256]), ([128, 256], [512, 256]), ([127, 129, 0, 255], [383, 385, 700, 257]),
-                                   ([640, 10, 700], [0, 3, 900]), ([2000], [2000]), ([1, 3, 5], [5000, 300, 1025])])
+                                   ([640, 10, 700], [0, 3, 900]), ([2000], [2000]), ([1, 3, 5], [5000, 300, 1025]),
+                                   ([1100, 3, 900], [1100, 1400, 900]), ([333] * 40, [333] * 40)])
 @pytest.mark.parametrize("causal", [False, True])
 def test_packed_long_lengths(gpu, nq, nk, causal):
     for d in (64, 128):
