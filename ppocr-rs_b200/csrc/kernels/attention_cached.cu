@@ -27,6 +27,8 @@
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
+#include <climits>
+
 #include "seq_common.cuh"
 
 namespace ppocr {
@@ -135,12 +137,32 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
     using Tiles = Ring<DP, FULL>;
     extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-    const int seq = blockIdx.x / splits, split = blockIdx.x % splits;
+    int seq = blockIdx.x / splits;
+    const int split = blockIdx.x % splits;
     const int group = p.heads / p.cache.kv_heads, parts = (group + kHeads - 1) / kHeads;
     const int kv = blockIdx.y / parts, part = blockIdx.y % parts;
     const int head0 = kv * group + part * kHeads, live_heads = min(kHeads, group - part * kHeads);
     const int page = p.cache.page, d = p.cache.d;
 
+    if (p.table.sequences <= kThreads) {
+        // Blocks start in the order of their numbers: the longest sequences come
+        // first, so that none is begun when the others are nearly done.  Thread i
+        // counts the sequences that come before sequence i.
+        int* lengths = reinterpret_cast<int*>(smem);
+        const int mine = threadIdx.x < p.table.sequences ? p.lengths[threadIdx.x] : INT_MIN;
+        lengths[threadIdx.x] = mine;
+        __syncthreads();
+        int before = 0;
+        for (int i = 0; i < p.table.sequences; ++i) {
+            const int other = lengths[i];
+            before += other > mine || (other == mine && i < threadIdx.x);
+        }
+        __syncthreads();
+        if (threadIdx.x < p.table.sequences && before == seq) lengths[0] = threadIdx.x;
+        __syncthreads();
+        seq = lengths[0];
+        __syncthreads();   // the rings take its place
+    }
     int len = p.lengths[seq];
     const long long room = (long long)p.table.width * page;
     if (len < 0 || len > room) {

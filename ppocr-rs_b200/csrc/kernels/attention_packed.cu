@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 5) atten
     const int n0 = warp * 16 + r;                  // this lane's rows: n0 and n0 + 8
     const int keys0 = keys_of(min(n0, rows - 1)), keys1 = keys_of(min(n0 + 8, rows - 1));
     const int sure = __reduce_min_sync(0xffffffffu, (unsigned)min(keys0, keys1));   // keys every row of the warp sees
+    const int most = n0 - r < rows ? (int)__reduce_max_sync(0xffffffffu, (unsigned)max(keys0, keys1)) : 0;
     float o[DT][4];
 #pragma unroll
     for (int i = 0; i < DT; ++i)
@@ -156,6 +157,13 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 5) atten
         __syncthreads();
         const T* kt = sk + (j & 1) * BN * P;
         const T* vt = sv + (j & 1) * BN * P;
+        // Eights of keys that some row of the warp sees (0 for a warp without
+        // rows): lines are short, and tiles seldom full.
+        const int left = min(NT, (most - j * BN + 7) / 8), seen = F32 && left > 0 ? NT : left;   // FP32: the whole tile is faster
+        if (seen <= 0) {
+            __syncthreads();
+            continue;
+        }
         float s[NT][4];
 #pragma unroll
         for (int i = 0; i < NT; ++i)
@@ -167,14 +175,16 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 5) atten
                 for (int i = 0; i < DP / 16; ++i) ldmatrix4(qf[i], sq + (warp * 16 + (lane & 15)) * P + i * 16 + (lane >> 4) * 8);
             }
 #pragma unroll
-            for (int i = 0; i < DP / 16; ++i)
+            for (int n = 0; n < NT; n += 2) {
+                if (n >= seen) break;
 #pragma unroll
-                for (int n = 0; n < NT; n += 2) {
+                for (int i = 0; i < DP / 16; ++i) {
                     uint32_t b[4];
                     ldmatrix4(b, kt + (n * 8 + (lane & 7) + (lane >> 4) * 8) * P + i * 16 + ((lane >> 3) & 1) * 8);
                     mma_bf16_16816(s[n], qf[i], b[0], b[1]);
                     mma_bf16_16816(s[n + 1], qf[i], b[2], b[3]);
                 }
+            }
         } else {
             // The tensor cores truncate when they add to an accumulator: the small
             // cross products are summed apart, the leading ones in chains of two.
@@ -193,6 +203,7 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 5) atten
                 split_tf32(qa[8 * P + 4], ah[3], al[3]);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
+                    if (n >= seen) break;
                     const float* kb = reinterpret_cast<const float*>(kt) + (n * 8 + r) * P + i * 8 + c;
                     uint32_t h0, e0, h1, e1;
                     split_tf32(kb[0], h0, e0);
@@ -216,7 +227,8 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 5) atten
         float t0 = -INFINITY, t1 = -INFINITY;
         const bool whole = (j + 1) * BN <= sure;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+            if (n >= (seen + 1) / 2 * 2) break;   // BF16 takes them in pairs
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const int key = j * BN + n * 8 + 2 * c + x;
@@ -225,6 +237,7 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 5) atten
                 t0 = fmaxf(t0, s[n][x]);
                 t1 = fmaxf(t1, s[n][x + 2]);
             }
+        }
         t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1));
         t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
         t0 = fmaxf(m0, fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2)));
@@ -242,6 +255,7 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 5) atten
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+            if (n >= (seen + 1) / 2 * 2) break;
             s[n][0] = exp2_hw(s[n][0] - b0); s[n][1] = exp2_hw(s[n][1] - b0);
             s[n][2] = exp2_hw(s[n][2] - b1); s[n][3] = exp2_hw(s[n][3] - b1);
             l0 += s[n][0] + s[n][1];
@@ -250,6 +264,7 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 5) atten
         if constexpr (!F32) {
 #pragma unroll
             for (int n = 0; n < NT; n += 2) {
+                if (n >= seen) break;
                 uint32_t a[4];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
@@ -281,6 +296,7 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 5) atten
                 float rest[4] = {0.f, 0.f, 0.f, 0.f}, part[4];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
+                    if (n >= (seen + 1) / 2 * 2) break;   // the sums' chains are of two
                     uint32_t h0, e0, h1, e1;
                     split_tf32(vb[n * 8 * P + i * 8], h0, e0);
                     split_tf32(vb[n * 8 * P + P + i * 8], h1, e1);

@@ -426,22 +426,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             }
             sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
         }
-        // A tile without keys still waits for its Q, whose place its output takes.
-        if (ok && live && steps > 0) wait(tiles > 0 ? &o_full[t] : &q_full, 0, 6);
+        if (ok && tiles > 0) wait(&o_full[t], 0, 6);
         if (ok && live) {
             // top: -infinity where every score is (or is no number), and then the
             // emulated weights are not quite 0.
             const float inv = sum == 0.f || (top == -INFINITY && !isnan(sum)) ? 0.f : 1.f / sum;
-            // Rows leave through shared memory (over the tile's Q, which the last
-            // scores have read), 16 bytes a lane along the row: stored as they lie
-            // in TMEM, a row per lane, they took 3,000 cycles.
-            uint8_t* stage = sq + t * DC * kQChunk;
-            auto piece = [&](int r, int x) { return stage + (x >> 3) * kQChunk + r * 128 + (((x & 7) ^ (r & 7)) << 4); };
+            const int token = w.qs.begin + w.token0 + t * w.per + row / w.group, head = w.kv * w.group + row % w.group;
+            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out.ptr) + token * p.out.token_stride + head * p.out.head_stride;
             bool bad = false;
-#pragma unroll 2
+            // Straight from TMEM, a row per lane.  (Through shared memory, with 512
+            // bytes to a store, it took 5,000 cycles instead of 3,000: the other
+            // tile's scores keep shared memory busy.)
             for (int c = 0; c < n_out; c += 16) {
-                uint32_t o[16] = {}, h[8];
+                uint32_t o[16] = {};
                 if (tiles > 0) tc::tmem_ld16(to + c, o);
+                if (row >= live) continue;
+                uint32_t h[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float x = __uint_as_float(o[2 * i]) * inv, y = __uint_as_float(o[2 * i + 1]) * inv;
@@ -449,27 +449,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                     const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
                     h[i] = *reinterpret_cast<const uint32_t*>(&v);
                 }
-                *reinterpret_cast<uint4*>(piece(row, c / 8)) = make_uint4(h[0], h[1], h[2], h[3]);
-                *reinterpret_cast<uint4*>(piece(row, c / 8 + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
-            }
-            bad &= row < live;
-            __syncwarp();
-            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out.ptr) + (long long)(w.qs.begin + w.token0 + t * w.per) * p.out.token_stride +
-                                 (long long)w.kv * w.group * p.out.head_stride;
-            const long long mine = (row / w.group) * p.out.token_stride + (row % w.group) * p.out.head_stride;
-            const int width = p.d / 8, shift = width > 8 ? 4 : width > 4 ? 3 : width > 2 ? 2 : width - 1;   // 2^shift lanes a row
-            for (int l0 = 0; l0 < 32; l0 += 32 >> shift) {
-                const int l = l0 + (lane >> shift), r = (warp & 3) * 32 + l, x = lane & ((1 << shift) - 1);
-                const long long off = __shfl_sync(0xffffffffu, mine, l);
-                if (r >= live || x >= width) continue;
-                const uint4 v = *reinterpret_cast<const uint4*>(piece(r, x));
-                if (vec_out) {
-                    *reinterpret_cast<uint4*>(out + off + x * 8) = v;
+                if (vec_out) {   // d is a multiple of 8
+                    *reinterpret_cast<uint4*>(out + c) = make_uint4(h[0], h[1], h[2], h[3]);
+                    if (c + 8 < p.d) *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(h[4], h[5], h[6], h[7]);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) out[off + x * 8 + i] = reinterpret_cast<const __nv_bfloat16*>(&v)[i];
+                    for (int i = 0; i < 16; ++i)
+                        if (c + i < p.d) out[c + i] = reinterpret_cast<const __nv_bfloat16*>(h)[i];
                 }
             }
+            __syncwarp();
             const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q.ptr);
             const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(p.k.ptr) + (long long)w.ks.begin * p.k.token_stride + w.kv * p.k.head_stride;
             const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(p.v.ptr) + (long long)w.ks.begin * p.v.token_stride + w.kv * p.v.head_stride;

@@ -19,33 +19,23 @@ namespace {
 
 constexpr int kThreads = 128;
 
-// Eight consecutive values, as one or two 16-byte loads when `vec`.
+// Eight consecutive values as they lie: 16 bytes of BF16, 32 of FP32, loaded 16
+// bytes at a time when `vec`.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, float (&x)[8]) {
-    if (vec) {
-        const float4 a = load4(p), b = load4(p + 4);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
+struct Raw8 {
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p, bool vec) {
+        if (vec) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = to_f(p[j]);
-    }
-}
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, bool vec, float (&x)[8]) {
-    if (vec) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        } else {
+            T* e = reinterpret_cast<T*>(w);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            x[2 * j] = __uint_as_float(w[j] << 16);
-            x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+            for (int j = 0; j < 8; ++j) e[j] = p[j];
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = to_f(p[j]);
     }
-}
+    __device__ __forceinline__ float operator[](int j) const { return to_f(reinterpret_cast<const T*>(w)[j]); }
+};
 
 template <typename T>
 __device__ __forceinline__ void store8(T* p, bool vec, const float (&x)[8]) {
@@ -58,21 +48,39 @@ __device__ __forceinline__ void store8(T* p, bool vec, const float (&x)[8]) {
     }
 }
 
-// round(a / s) of the exact quotient, ties to even, clamped to +-127; 0 for a
-// scale of 0 or a quotient that is no number.  t = a (1 / s) in FP32 is within
-// 2^-15 of the quotient (|a / s| <= 128, three roundings of 2^-24), so unless
-// t lies that near to a half it rounds as the quotient does; the few that do
-// are divided in FP64, which is exact at a tie.
-__device__ __forceinline__ int round_quotient(float a, float s, float inv) {
-    if (!(s > 0.f)) return 0;
-    const float t = a * inv;
-    float r = rintf(t);
-    if (!(fabsf(fabsf(t - r) - 0.5f) > 1.f / 8192.f) || !(fabsf(t) < 256.f)) {
-        const double d = (double)a / (double)s;
-        if (!(fabs(d) < 1e9)) return 0;
-        r = (float)rint(d);
+// Integers of eight values of a page with scale s: round(a / s) of the exact
+// quotient, ties to even; 0 for a scale of 0 or a quotient that is no number.
+__device__ __noinline__ uint2 exact_round8(const float (&x)[8], float s) {
+    uint2 u = make_uint2(0, 0);
+#pragma unroll 1
+    for (int j = 0; j < 8; ++j) {
+        const double d = s > 0.f ? (double)x[j] / (double)s : 0.0;
+        const int q = fabs(d) < 1e9 ? (int)fmin(fmax(rint(d), -127.0), 127.0) : 0;
+        (j < 4 ? u.x : u.y) |= (uint32_t)(q & 0xff) << (8 * (j & 3));
     }
-    return (int)fminf(fmaxf(r, -127.f), 127.f);
+    return u;
+}
+// t = a (1 / s) in FP32 is within 2^-15 of the quotient (|a / s| <= 127, two
+// roundings of 2^-24 each), so unless a t lies within 2^-13 of a half it rounds
+// as the quotient does; eights with one that does, and pages whose scale has no
+// ordinary reciprocal (`inv` 0), are divided in FP64, which is exact at a tie.
+// Adding 1.5 x 2^23 rounds to an integer whose low byte is the sum's.
+__device__ __forceinline__ uint2 round8(const float (&x)[8], float s, float inv) {
+    constexpr float kMagic = 12582912.f;
+    float y[8], rest = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float t = x[j] * inv;
+        y[j] = t + kMagic;
+        rest = fmaxf(rest, fabsf(t - (y[j] - kMagic)));
+    }
+    if (inv == 0.f || rest > 0.5f - 1.f / 8192.f) return exact_round8(x, s);
+    auto low = [&](int j) {
+        const uint32_t a = __byte_perm(__float_as_uint(y[j]), __float_as_uint(y[j + 1]), 0x0040);
+        const uint32_t b = __byte_perm(__float_as_uint(y[j + 2]), __float_as_uint(y[j + 3]), 0x0040);
+        return __byte_perm(a, b, 0x5410);
+    };
+    return make_uint2(low(0), low(4));
 }
 
 __device__ __forceinline__ uint2 pack8(const int (&q)[8]) {
@@ -84,7 +92,7 @@ __device__ __forceinline__ uint2 pack8(const int (&q)[8]) {
 
 // One block per (touched page, head, K or V).
 template <typename T>
-__global__ void __launch_bounds__(kThreads) cache_append_kernel(CacheAppendParams p, bool vec) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 8 : 7) cache_append_kernel(CacheAppendParams p, bool vec) {
     __shared__ uint32_t top[kThreads / 32];
     // A sequence's n new tokens touch at most n / page + 2 pages.
     const int page = p.cache.page, d8 = p.cache.d / 8, head = blockIdx.y;
@@ -120,21 +128,37 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(CacheAppendParam
     // floats order as the floats do, with infinity and NaN on top, so a NaN
     // marks its page's scale instead of getting lost.
     constexpr int KEEP = 4;
-    float kept[KEEP][8];
-    const int items = fresh * d8;
+    Raw8<T> kept[KEEP];
+    // Item i is eights i % d8 of token i / d8; a thread's items are kThreads apart.
+    const int step_row = kThreads / d8, step_col = kThreads % d8, row0 = threadIdx.x / d8, col0 = threadIdx.x % d8;
+    auto next = [&](int& row, int& col) {
+        row += step_row;
+        col += step_col;
+        if (col >= d8) {
+            col -= d8;
+            ++row;
+        }
+    };
     uint32_t amax = 0;
+    int row = row0, col = col0;
 #pragma unroll
     for (int n = 0; n < KEEP; ++n) {
-        const int i = threadIdx.x + n * kThreads;
-        if (i < items) {
-            load8(in + (i / d8) * src.token_stride + (i % d8) * 8, vec, kept[n]);
+        if (row < fresh) kept[n].load(in + row * src.token_stride + col * 8, vec);
+        next(row, col);
+    }
+    row = row0;
+    col = col0;
+#pragma unroll
+    for (int n = 0; n < KEEP; ++n) {
+        if (row < fresh) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(kept[n][j]) & 0x7fffffffu);
         }
+        next(row, col);
     }
-    for (int i = threadIdx.x + KEEP * kThreads; i < items; i += kThreads) {
-        float x[8];
-        load8(in + (i / d8) * src.token_stride + (i % d8) * 8, vec, x);
+    for (int r = row, c = col; r < fresh; next(r, c)) {
+        Raw8<T> x;
+        x.load(in + r * src.token_stride + c * 8, vec);
 #pragma unroll
         for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(x[j]) & 0x7fffffffu);
     }
@@ -145,7 +169,7 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(CacheAppendParam
     for (int w = 0; w < kThreads / 32; ++w) amax = max(amax, top[w]);
     const float mine = __uint_as_float(amax) * (1.f / 127.f);
     const float now = __uint_as_float(max(__float_as_uint(mine) & 0x7fffffffu, __float_as_uint(before) & 0x7fffffffu));
-    const float inv = 1.f / now;
+    const float inv = now > 1e-30f && now < 1e30f ? 1.f / now : 0.f;
     if (threadIdx.x == 0) *scale = now;
 
     if (old && now > before) {
@@ -164,68 +188,88 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(CacheAppendParam
         }
     }
     uint2* dst = reinterpret_cast<uint2*>(out + (long long)old * p.cache.d);
+    auto store = [&](int r, int c, const Raw8<T>& raw) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = raw[j];
+        dst[r * d8 + c] = round8(x, now, inv);
+    };
+    row = row0;
+    col = col0;
 #pragma unroll
     for (int n = 0; n < KEEP; ++n) {
-        const int i = threadIdx.x + n * kThreads;
-        if (i < items) {
-            int q[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) q[j] = round_quotient(kept[n][j], now, inv);
-            dst[i] = pack8(q);
-        }
+        if (row < fresh) store(row, col, kept[n]);
+        next(row, col);
     }
-    for (int i = threadIdx.x + KEEP * kThreads; i < items; i += kThreads) {
-        float x[8];
-        load8(in + (i / d8) * src.token_stride + (i % d8) * 8, vec, x);
-        int q[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) q[j] = round_quotient(x[j], now, inv);
-        dst[i] = pack8(q);
+    for (; row < fresh; next(row, col)) {
+        Raw8<T> x;
+        x.load(in + row * src.token_stride + col * 8, vec);
+        store(row, col, x);
     }
 }
 
-// Tokens per block of the read kernel.
-constexpr int kReadTokens = 8;
+// Tokens per block of the read kernel, and values in flight per thread.
+constexpr int kReadTokens = 16, kReadThreads = 256, kReadAhead = 4;
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) cache_read_kernel(CacheReadParams p, bool vec) {
+__global__ void __launch_bounds__(kReadThreads) cache_read_kernel(CacheReadParams p, bool vec) {
     __shared__ int where[kReadTokens], slot[kReadTokens];
-    const int t0 = blockIdx.x * kReadTokens;
+    const int t0 = blockIdx.x * kReadTokens, lane = threadIdx.x & 31;
     const int tokens = min(kReadTokens, p.total - t0);
-    if (threadIdx.x < tokens) {
-        // The sequence of the token: the last one whose offset is not past it.
-        const int t = t0 + threadIdx.x;
-        int lo = 0, hi = p.table.sequences;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (p.offsets[mid] <= t) lo = mid; else hi = mid;
-        }
-        where[threadIdx.x] = -1;
-        if (t >= p.offsets[lo] && t < p.offsets[lo + 1]) {
-            const long long at = (long long)p.first[lo] + (t - p.offsets[lo]);
-            if (p.first[lo] >= 0 && at < (long long)p.table.width * p.cache.page) {
-                const int w = p.table.pages[lo * p.table.stride + at / p.cache.page];
-                if (w >= 0 && w < p.cache.pages) where[threadIdx.x] = w;
-                slot[threadIdx.x] = (int)(at % p.cache.page);
+    for (int i = threadIdx.x / 32; i < tokens; i += kReadThreads / 32) {
+        const int t = t0 + i, seq = find_owner(p.table.sequences, t, [&](int s) { return seq_offset(p.offsets, 0, s, p.total); });
+        // Sequences without tokens start where the next one does: the last one is the owner.
+        const int begin = p.offsets[seq], end = p.offsets[seq + 1], first = p.first[seq];
+        int w = -1, at = 0;
+        if (t >= begin && t < end) {
+            const long long pos = (long long)first + (t - begin);
+            if (first >= 0 && pos < (long long)p.table.width * p.cache.page) {
+                w = p.table.pages[seq * p.table.stride + pos / p.cache.page];
+                at = (int)(pos % p.cache.page);
             }
-            if (where[threadIdx.x] < 0) seq_bad_index(p.status);
+            if (w < 0 || w >= p.cache.pages) {
+                w = -1;
+                if (lane == 0) seq_bad_index(p.status);
+            }
+        }
+        if (lane == 0) {
+            where[i] = w;
+            slot[i] = at;
         }
     }
     __syncthreads();
+    // A thread keeps its place in a token (head and eight) and takes every n-th
+    // token; places beyond the threads' number in further rounds.
     const int d8 = p.cache.d / 8, per = p.cache.kv_heads * d8;
     const int8_t* pages = blockIdx.y ? p.cache.v : p.cache.k;
     const float* scales = blockIdx.y ? p.cache.v_scales : p.cache.k_scales;
     const SeqTensor& dst = blockIdx.y ? p.v : p.k;
-    for (int i = threadIdx.x; i < tokens * per; i += kThreads) {
-        const int t = i / per, head = (i % per) / d8, c = i % d8;
-        if (where[t] < 0) continue;
-        const long long cell = (long long)where[t] * p.cache.kv_heads + head;
-        const float s = __ldg(scales + cell);
-        const uint2 u = __ldcs(reinterpret_cast<const uint2*>(pages + (cell * p.cache.page + slot[t]) * p.cache.d) + c);
-        float x[8];
+    const int every = max(1, kReadThreads / per), mine = every > 1 ? threadIdx.x / per : 0;
+    if (mine >= every) return;
+    for (int place = every > 1 ? threadIdx.x % per : threadIdx.x; place < per; place += kReadThreads) {
+        const int head = place / d8, c = place % d8;
+        const long long in_at = (long long)head * p.cache.page * p.cache.d + c * 8, out_at = head * dst.head_stride + c * 8;
+        for (int i0 = mine; i0 < tokens; i0 += every * kReadAhead) {
+            uint2 u[kReadAhead];
+            float s[kReadAhead];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = (float)(int8_t)((j < 4 ? u.x : u.y) >> (8 * (j & 3))) * s;
-        store8(static_cast<T*>(dst.ptr) + (t0 + t) * dst.token_stride + head * dst.head_stride + c * 8, vec, x);
+            for (int n = 0; n < kReadAhead; ++n) {
+                const int i = i0 + n * every;
+                if (i >= tokens || where[i] < 0) continue;
+                s[n] = __ldg(scales + (long long)where[i] * p.cache.kv_heads + head);
+                u[n] = __ldcs(reinterpret_cast<const uint2*>(
+                    pages + ((long long)where[i] * p.cache.kv_heads * p.cache.page + slot[i]) * p.cache.d + in_at));
+            }
+#pragma unroll
+            for (int n = 0; n < kReadAhead; ++n) {
+                const int i = i0 + n * every;
+                if (i >= tokens || where[i] < 0) continue;
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = (float)(int8_t)((j < 4 ? u[n].x : u[n].y) >> (8 * (j & 3))) * s[n];
+                store8(static_cast<T*>(dst.ptr) + (t0 + i) * dst.token_stride + out_at, vec, x);
+            }
+        }
     }
 }
 
@@ -252,8 +296,8 @@ cudaError_t launch_cache_read(const CacheReadParams& p, cudaStream_t stream) {
     const int esize = (int)dtype_size(p.dtype);
     const bool vec = vec8(p.k, esize) && vec8(p.v, esize);
     const dim3 grid((p.total + kReadTokens - 1) / kReadTokens, 2);
-    if (p.dtype == DT_F32) cache_read_kernel<float><<<grid, kThreads, 0, stream>>>(p, vec);
-    else cache_read_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(p, vec);
+    if (p.dtype == DT_F32) cache_read_kernel<float><<<grid, kReadThreads, 0, stream>>>(p, vec);
+    else cache_read_kernel<__nv_bfloat16><<<grid, kReadThreads, 0, stream>>>(p, vec);
     return cudaGetLastError();
 }
 

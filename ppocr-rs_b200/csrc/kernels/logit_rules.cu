@@ -43,79 +43,107 @@ __device__ __forceinline__ const uint32_t* mask_row(const LogitRulesParams& p, i
     return p.mask + (long long)state * p.mask_ld;
 }
 
-// Rows are independent and without a history: block (x, y) holds columns
-// [x, x + 1) x kThreads x VEC and rows y, y + gridDim.y, ...; four rows are in
-// flight per thread so that each SM has enough loads outstanding.
+// Rows without a history: a block holds COLS vectors of columns per thread
+// and rows y, y + gridDim.y, ...; kRowsAhead rows of them are in flight per
+// thread, so that each SM has enough loads outstanding and what a row costs
+// besides (its mask's state, addresses) is shared by the vectors.
+constexpr int kRowsAhead = 4;
+template <int VEC> constexpr int kRowCols = VEC == 8 ? 1 : 2;   // more would not fit the registers
+
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) logit_rules_rows_kernel(LogitRulesParams p) {
+__global__ void __launch_bounds__(kThreads, 5) logit_rules_rows_kernel(LogitRulesParams p) {
+    constexpr int COLS = kRowCols<VEC>;
     using V = typename VecType<T, VEC>::type;
-    constexpr int ROWS = 4;
-    const int v = (blockIdx.x * kThreads + threadIdx.x) * VEC;
-    if (v >= p.vocab) return;
-    const int live = min(VEC, p.vocab - v);
-    float bias[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) bias[j] = p.bias && j < live ? __ldg(p.bias + v + j) : 0.f;
+    const int v0 = (blockIdx.x * kThreads * COLS + threadIdx.x) * VEC;
+    float bias[COLS][VEC];
+    uint32_t bits0[COLS];
     const bool shared = !p.mask_index;
-    const uint32_t bits0 = p.mask && shared ? mask_bits(p.mask, v) : ~0u;
-    const T* in = static_cast<const T*>(p.logits) + v;
-    T* out = static_cast<T*>(p.out) + v;
-    for (int r0 = blockIdx.y; r0 < p.rows; r0 += ROWS * gridDim.y) {
-        V x[ROWS];
-        uint32_t bits[ROWS];
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-            const int r = r0 + i * gridDim.y;
-            bits[i] = bits0;
+    for (int c = 0; c < COLS; ++c) {
+        const int v = v0 + c * kThreads * VEC;
+        bits0[c] = p.mask && shared && v < p.vocab ? mask_bits(p.mask, v) : ~0u;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) bias[c][j] = p.bias && v + j < p.vocab ? __ldg(p.bias + v + j) : 0.f;
+    }
+    for (int r0 = blockIdx.y; r0 < p.rows; r0 += kRowsAhead * (int)gridDim.y) {
+        V x[kRowsAhead][COLS];
+        uint32_t bits[kRowsAhead][COLS];
+#pragma unroll
+        for (int i = 0; i < kRowsAhead; ++i) {
+            const int r = r0 + i * (int)gridDim.y;
             if (r >= p.rows) continue;
-            const T* src = in + r * p.ld;
-            if (live == VEC) {
-                x[i] = __ldcs(reinterpret_cast<const V*>(src));
-            } else {
-                T* e = reinterpret_cast<T*>(&x[i]);
+            const T* in = static_cast<const T*>(p.logits) + r * p.ld;
+            const uint32_t* m = shared ? nullptr : mask_row(p, r);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    if (j < live) e[j] = src[j];
-            }
-            if (!shared) {
-                const uint32_t* m = mask_row(p, r);
-                if (m) bits[i] = mask_bits(m, v);
+            for (int c = 0; c < COLS; ++c) {
+                const int v = v0 + c * kThreads * VEC;
+                bits[i][c] = shared ? bits0[c] : m && v < p.vocab ? mask_bits(m, v) : ~0u;
+                if (v + VEC <= p.vocab) {
+                    x[i][c] = __ldcs(reinterpret_cast<const V*>(in + v));
+                } else {
+                    T* e = reinterpret_cast<T*>(&x[i][c]);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j)
+                        if (v + j < p.vocab) e[j] = in[v + j];
+                }
             }
         }
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-            const int r = r0 + i * gridDim.y;
+        for (int i = 0; i < kRowsAhead; ++i) {
+            const int r = r0 + i * (int)gridDim.y;
             if (r >= p.rows) continue;
-            T* e = reinterpret_cast<T*>(&x[i]);
+            T* out = static_cast<T*>(p.out) + r * p.out_ld;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float y = to_f(e[j]) + bias[j];
-                e[j] = from_f<T>((bits[i] >> j) & 1u ? y : -INFINITY);
-            }
-            T* dst = out + r * p.out_ld;
-            if (live == VEC) {
-                __stcs(reinterpret_cast<V*>(dst), x[i]);
-            } else {
+            for (int c = 0; c < COLS; ++c) {
+                const int v = v0 + c * kThreads * VEC;
+                T* e = reinterpret_cast<T*>(&x[i][c]);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    if (j < live) dst[j] = e[j];
+                for (int j = 0; j < VEC; ++j) {
+                    const float y = to_f(e[j]) + bias[c][j];
+                    e[j] = from_f<T>((bits[i][c] >> j) & 1u ? y : -INFINITY);
+                }
+                if (v + VEC <= p.vocab) {
+                    __stcs(reinterpret_cast<V*>(out + v), x[i][c]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j)
+                        if (v + j < p.vocab) out[v + j] = e[j];
+                }
             }
         }
     }
 }
 
-// One chunk of one row with a history.
+// One chunk of one row with a history.  The first kAhead vectors of logits are
+// on their way while the history is counted.
+constexpr int kRowThreads = 512, kAhead = 4;
+
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) logit_rules_history_kernel(LogitRulesParams p, int chunk) {
+__global__ void __launch_bounds__(kRowThreads) logit_rules_history_kernel(LogitRulesParams p, int chunk) {
     using V = typename VecType<T, VEC>::type;
-    extern __shared__ uint32_t counts[];
+    extern __shared__ uint4 counts4[];
+    uint32_t* counts = reinterpret_cast<uint32_t*>(counts4);
     const int row = blockIdx.y, lo = blockIdx.x * chunk, hi = min(lo + chunk, p.vocab);
+    const T* in = static_cast<const T*>(p.logits) + row * p.ld;
+    T* out = static_cast<T*>(p.out) + row * p.out_ld;
+    auto load = [&](int v) {
+        V x;
+        if (v + VEC <= hi) return __ldcs(reinterpret_cast<const V*>(in + v));
+        T* e = reinterpret_cast<T*>(&x);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) e[j] = v + j < hi ? in[v + j] : from_f<T>(0.f);
+        return x;
+    };
+    V ahead[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ahead[i] = load(lo + (threadIdx.x + i * kRowThreads) * VEC);
     const Span h = seq_span(p.history_offsets, 0, row, p.history_total, p.status);
     const bool any = h.len > 0;
     if (any) {
-        for (int i = threadIdx.x; i < hi - lo; i += kThreads) counts[i] = 0;
+        for (int i = threadIdx.x; i < (hi - lo + 3) / 4; i += kRowThreads) counts4[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        for (int i = threadIdx.x; i < h.len; i += kThreads) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < h.len; i += kRowThreads) {
             const int id = __ldg(p.history + h.begin + i);
             if (id >= lo && id < hi) atomicAdd(&counts[id - lo], 1u);
             else if (id < 0 || id >= p.vocab) seq_bad_index(p.status);
@@ -126,30 +154,46 @@ __global__ void __launch_bounds__(kThreads) logit_rules_history_kernel(LogitRule
     const float pres = p.presence ? p.presence[row] : 0.f;
     const float freq = p.frequency ? p.frequency[row] : 0.f;
     const uint32_t* mask = mask_row(p, row);
-    const T* in = static_cast<const T*>(p.logits) + row * p.ld;
-    T* out = static_cast<T*>(p.out) + row * p.out_ld;
-    for (int v = lo + threadIdx.x * VEC; v < hi; v += kThreads * VEC) {
+    const bool bias4 = (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0;
+    auto apply = [&](int v, V x) {
         const int live = min(VEC, hi - v);
-        V x;
         T* e = reinterpret_cast<T*>(&x);
-        if (live == VEC) {
-            x = __ldcs(reinterpret_cast<const V*>(in + v));
-        } else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (j < live) e[j] = in[v + j];
-        }
         const uint32_t bits = mask ? mask_bits(mask, v) : ~0u;
+        // Bias and counts by fours where VEC has fours: a lane's neighbours are
+        // VEC words on, so single words would meet in the same banks and sectors.
+        alignas(16) float bias[VEC];
+        alignas(16) uint32_t n[VEC];
+        constexpr int Q = VEC >= 4 ? VEC / 4 : 1;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            if (j >= live) continue;
-            float y = to_f(e[j]);
-            const uint32_t n = any ? counts[v - lo + j] : 0u;
-            if (n) {
-                y = y > 0.f ? y / rep : y * rep;
-                y = y - freq * (float)n - pres;
+            bias[j] = 0.f;
+            n[j] = 0;
+        }
+        if (VEC >= 4 && live == VEC && bias4) {
+            if (p.bias) {
+#pragma unroll
+                for (int q = 0; q < Q; ++q) *reinterpret_cast<float4*>(bias + 4 * q) = __ldg(reinterpret_cast<const float4*>(p.bias + v) + q);
             }
-            if (p.bias) y += __ldg(p.bias + v + j);
+            if (any) {
+#pragma unroll
+                for (int q = 0; q < Q; ++q) *reinterpret_cast<uint4*>(n + 4 * q) = counts4[(v - lo) / 4 + q];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                if (j >= live) continue;
+                if (p.bias) bias[j] = __ldg(p.bias + v + j);
+                if (any) n[j] = counts[v - lo + j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            float y = to_f(e[j]);
+            if (n[j]) {
+                y = y > 0.f ? y / rep : y * rep;
+                y = y - freq * (float)n[j] - pres;
+            }
+            y += bias[j];
             e[j] = from_f<T>((bits >> j) & 1u ? y : -INFINITY);
         }
         if (live == VEC) {
@@ -159,20 +203,32 @@ __global__ void __launch_bounds__(kThreads) logit_rules_history_kernel(LogitRule
             for (int j = 0; j < VEC; ++j)
                 if (j < live) out[v + j] = e[j];
         }
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        const int v = lo + (threadIdx.x + i * kRowThreads) * VEC;
+        if (v < hi) apply(v, ahead[i]);
     }
+    for (int v = lo + (threadIdx.x + kAhead * kRowThreads) * VEC; v < hi; v += kRowThreads * VEC) apply(v, load(v));
 }
 
 template <typename T, int VEC>
 cudaError_t launch_vec(const LogitRulesParams& p, cudaStream_t stream) {
     if (!p.history_offsets) {
-        const int gx = (p.vocab + kThreads * VEC - 1) / (kThreads * VEC);
-        // About eight blocks per SM in all, and no more than one row group each.
-        const int gy = max(1, min((p.rows + 3) / 4, (148 * 8 + gx - 1) / gx));
+        const int width = kThreads * VEC * kRowCols<VEC>, gx = (p.vocab + width - 1) / width;
+        // One wave of five blocks per SM (a second, short one would double the
+        // time), and no more than one group of rows each.
+        const int gy = max(1, min((p.rows + kRowsAhead - 1) / kRowsAhead, 148 * 5 / gx));
         logit_rules_rows_kernel<T, VEC><<<dim3(gx, gy), kThreads, 0, stream>>>(p);
         return cudaGetLastError();
     }
-    // A chunk's counts fit 16 KB, so the blocks of an SM are bound by threads.
-    const int chunk = 4096;
+    // Every block of a row reads the row's whole history, so a row is cut into
+    // as few chunks as give about three blocks per SM, of 1,024 to 16,384
+    // classes (64 KB of counts).
+    const int parts = max((p.vocab + 16383) / 16384, min((p.vocab + 1023) / 1024, max(1, 148 * 3 / p.rows)));
+    const int chunk = ((p.vocab + parts - 1) / parts + 63) / 64 * 64, smem = chunk * (int)sizeof(uint32_t);
+    cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(logit_rules_history_kernel<T, VEC>), 16384 * 4);
+    if (e != cudaSuccess) return e;
     for (int r0 = 0; r0 < p.rows; r0 += 65535) {
         LogitRulesParams q = p;
         q.rows = min(65535, p.rows - r0);
@@ -183,8 +239,7 @@ cudaError_t launch_vec(const LogitRulesParams& p, cudaStream_t stream) {
         if (p.presence) q.presence = p.presence + r0;
         if (p.frequency) q.frequency = p.frequency + r0;
         if (p.mask_index) q.mask_index = p.mask_index + r0;
-        logit_rules_history_kernel<T, VEC><<<dim3((p.vocab + chunk - 1) / chunk, q.rows), kThreads,
-                                             chunk * sizeof(uint32_t), stream>>>(q, chunk);
+        logit_rules_history_kernel<T, VEC><<<dim3((p.vocab + chunk - 1) / chunk, q.rows), kRowThreads, smem, stream>>>(q, chunk);
     }
     return cudaGetLastError();
 }
