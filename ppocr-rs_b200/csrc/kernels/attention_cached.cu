@@ -61,6 +61,15 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same onto zeros: the first step of a chain.
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                              uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 __device__ __forceinline__ void add4(float (&a)[4], const float (&b)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] += b[i];
@@ -88,9 +97,9 @@ struct Ring {
 
     // Starts the copies of slots slot0 .. slot0 + 15 of `head` of page `where`.
     static __device__ __forceinline__ void fetch(const CachedAttentionParams& p, uint32_t stage, int where, int head, int slot0,
-                                                 int lane) {
+                                                 int page_bytes, int lane) {
         const int d = FULL ? DP : p.cache.d;
-        const long long cell = (long long)where * p.cache.kv_heads + head, at0 = (cell * p.cache.page + slot0) * d;
+        const long long cell = (long long)where * p.cache.kv_heads + head, at0 = cell * page_bytes + slot0 * d;
         const int8_t* kp = p.cache.k + at0;
         const int8_t* vp = p.cache.v + at0;
 #pragma unroll
@@ -196,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
         for (int h = 0; h < kPair; ++h) {
             if (w_ahead[h] >= 0)
                 Tiles::fetch(p, ring + stage_ahead * Tiles::kStage + h * Tiles::kOne, w_ahead[h], kv,
-                             (ahead * kPair + h) * kTile & (page - 1), lane);
+                             (ahead * kPair + h) * kTile & (page - 1), page * d, lane);
             else
                 missing |= 1u << (kPair * stage_ahead + h);
         }
@@ -271,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
 #pragma unroll
         for (int h = 0; h < kPair; ++h) {
             uint32_t k[2][DP / 16];
-            float sk, rest[4] = {0.f, 0.f, 0.f, 0.f}, part[4];
+            float sk, rest[4], part[4];
             asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(sk), "=f"(sv[h]) : "r"(at + h * Tiles::kOne + 2 * Tiles::kRows));
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -280,17 +289,20 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
                     read_words<PK>(at + h * Tiles::kOne + k_at + 8 * i * DP + Tiles::k_chunk(r, (c * PK >> 4) + 4 * j) * 16 +
                                        (c * PK & 15),
                                    &k[i][j * PK / 4]);
-            s[h][0] = s[h][1] = s[h][2] = s[h][3] = 0.f;
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
                 const uint32_t u0 = k[0][i] ^ 0x80808080u, u1 = k[1][i] ^ 0x80808080u;
                 const uint32_t a0 = bytes_to_h2(u0, 0x4140), a1 = bytes_to_h2(u1, 0x4140);
                 const uint32_t a2 = bytes_to_h2(u0, 0x4342), a3 = bytes_to_h2(u1, 0x4342);
                 if constexpr (SPLIT) {
-                    if (i % 2 == 0) part[0] = part[1] = part[2] = part[3] = 0.f;
-                    mma_f16(part, a0, a1, a2, a3, qh[i][0], qh[i][1]);
-                    mma_f16(rest, a0, a1, a2, a3, ql[i][0], ql[i][1]);
-                    if (i % 2 == 1) add4(s[h], part);
+                    if (i == 0) mma_f16_first(rest, a0, a1, a2, a3, ql[i][0], ql[i][1]);
+                    else mma_f16(rest, a0, a1, a2, a3, ql[i][0], ql[i][1]);
+                    float (&sum)[4] = i < 2 ? s[h] : part;
+                    if (i % 2 == 0) mma_f16_first(sum, a0, a1, a2, a3, qh[i][0], qh[i][1]);
+                    else mma_f16(sum, a0, a1, a2, a3, qh[i][0], qh[i][1]);
+                    if (i > 2 && i % 2 == 1) add4(s[h], part);
+                } else if (i == 0) {
+                    mma_f16_first(s[h], a0, a1, a2, a3, qh[i][0], qh[i][1]);
                 } else {
                     mma_f16(s[h], a0, a1, a2, a3, qh[i][0], qh[i][1]);
                 }
@@ -366,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
         for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                float sum[4];
 #pragma unroll
                 for (int h = 0; h < kPair; ++h) {
                     // Bytes 2b and 2b + 1 of two tokens, interleaved by value of d.
@@ -375,7 +387,8 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
                     const uint32_t a0 = bytes_to_h2(x, 0x4140), a1 = bytes_to_h2(x, 0x4342);
                     const uint32_t a2 = bytes_to_h2(y, 0x4140), a3 = bytes_to_h2(y, 0x4342);
                     if constexpr (SPLIT) {   // a pair's sum apart, added to the running one with rounding
-                        mma_f16(sum, a0, a1, a2, a3, e0[h], e1[h]);
+                        if (h == 0) mma_f16_first(sum, a0, a1, a2, a3, e0[h], e1[h]);
+                        else mma_f16(sum, a0, a1, a2, a3, e0[h], e1[h]);
                         mma_f16(sum, a0, a1, a2, a3, p0[h], p1[h]);
                     } else {
                         mma_f16(o[2 * i + b], a0, a1, a2, a3, p0[h], p1[h]);

@@ -19,24 +19,6 @@ namespace {
 
 constexpr int kThreads = 128;
 
-// Eight consecutive values as they lie: 16 bytes of BF16, 32 of FP32, loaded 16
-// bytes at a time when `vec`.
-template <typename T>
-struct Raw8 {
-    uint4 w[sizeof(T) / 2];
-    __device__ __forceinline__ void load(const T* p, bool vec) {
-        if (vec) {
-#pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-        } else {
-            T* e = reinterpret_cast<T*>(w);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] = p[j];
-        }
-    }
-    __device__ __forceinline__ float operator[](int j) const { return to_f(reinterpret_cast<const T*>(w)[j]); }
-};
-
 template <typename T>
 __device__ __forceinline__ void store8(T* p, bool vec, const float (&x)[8]) {
     if (vec) {
@@ -48,39 +30,47 @@ __device__ __forceinline__ void store8(T* p, bool vec, const float (&x)[8]) {
     }
 }
 
-// Integers of eight values of a page with scale s: round(a / s) of the exact
-// quotient, ties to even; 0 for a scale of 0 or a quotient that is no number.
-__device__ __noinline__ uint2 exact_round8(const float (&x)[8], float s) {
-    uint2 u = make_uint2(0, 0);
-#pragma unroll 1
-    for (int j = 0; j < 8; ++j) {
-        const double d = s > 0.f ? (double)x[j] / (double)s : 0.0;
-        const int q = fabs(d) < 1e9 ? (int)fmin(fmax(rint(d), -127.0), 127.0) : 0;
-        (j < 4 ? u.x : u.y) |= (uint32_t)(q & 0xff) << (8 * (j & 3));
-    }
-    return u;
-}
-// t = a (1 / s) in FP32 is within 2^-15 of the quotient (|a / s| <= 127, two
-// roundings of 2^-24 each), so unless a t lies within 2^-13 of a half it rounds
-// as the quotient does; eights with one that does, and pages whose scale has no
-// ordinary reciprocal (`inv` 0), are divided in FP64, which is exact at a tie.
-// Adding 1.5 x 2^23 rounds to an integer whose low byte is the sum's.
-__device__ __forceinline__ uint2 round8(const float (&x)[8], float s, float inv) {
+// The integers of eight values of a page with scale s: round(a / s) of the exact
+// quotient, ties to even.  With r = round(a inv), inv = 1 / s, the remainder
+// a - r s is a multiple of half the last place of s and not much above s / 2,
+// so a fused multiply-add gives it exactly; r moves by one towards it where it
+// is more than s / 2, or just that and r is odd (as integers the bit patterns of
+// positive floats compare as the floats do).  No branch: values of half a page's
+// largest are common, and their quotient is 63.5.  Adding 1.5 x 2^23 rounds to
+// an integer whose low byte is the sum's.
+template <typename T>
+__device__ __forceinline__ uint2 round8(const Pack<T, 8>& x, float s, float inv) {
     constexpr float kMagic = 12582912.f;
-    float y[8], rest = 0.f;
+    const int half = __float_as_int(0.5f * s);
+    float y[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const float t = x[j] * inv;
-        y[j] = t + kMagic;
-        rest = fmaxf(rest, fabsf(t - (y[j] - kMagic)));
+        const float a = x.get(j);
+        y[j] = fmaf(a, inv, kMagic);
+        const int e = __float_as_int(fmaf(kMagic - y[j], s, a));
+        if ((e & 0x7fffffff) + (__float_as_int(y[j]) & 1) > half) y[j] += __int_as_float((e & 0x80000000) | 0x3f800000);
     }
-    if (inv == 0.f || rest > 0.5f - 1.f / 8192.f) return exact_round8(x, s);
     auto low = [&](int j) {
         const uint32_t a = __byte_perm(__float_as_uint(y[j]), __float_as_uint(y[j + 1]), 0x0040);
         const uint32_t b = __byte_perm(__float_as_uint(y[j + 2]), __float_as_uint(y[j + 3]), 0x0040);
         return __byte_perm(a, b, 0x5410);
     };
     return make_uint2(low(0), low(4));
+}
+
+// The same for a scale without an ordinary reciprocal, in FP64; 0 for a scale of
+// 0 or a quotient that is no number.
+template <typename T>
+__device__ __noinline__ uint2 round8_odd(const T* p, float s) {
+    uint2 u = make_uint2(0, 0);
+#pragma unroll 1
+    for (int j = 0; j < 8; ++j) {
+        const double d = s > 0.f ? (double)to_f(p[j]) / (double)s : 0.0;
+        const int q = fabs(d) < 1e9 ? (int)fmin(fmax(rint(d), -127.0), 127.0) : 0;
+        const uint32_t byte = (uint32_t)(q & 0xff) << (8 * (j & 3));
+        if (j < 4) u.x |= byte; else u.y |= byte;
+    }
+    return u;
 }
 
 __device__ __forceinline__ uint2 pack8(const int (&q)[8]) {
@@ -95,7 +85,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 8 : 7) cache_append_kernel(CacheAppendParams p, bool vec) {
     __shared__ uint32_t top[kThreads / 32];
     // A sequence's n new tokens touch at most n / page + 2 pages.
-    const int page = p.cache.page, d8 = p.cache.d / 8, head = blockIdx.y;
+    const int page = p.cache.page, d8 = p.cache.d / 8;
     const int page_shift = 31 - __clz(page), id = blockIdx.x;
     auto first_id = [&](int i) { return (seq_offset(p.offsets, 0, i, p.total) >> page_shift) + 2 * i; };
     const int seq = find_owner(p.table.sequences, id, first_id);
@@ -118,18 +108,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 8 : 7) cache_append
         return;
     }
     const SeqTensor& src = blockIdx.z ? p.v : p.k;
-    const T* in = static_cast<const T*>(src.ptr) + (span.begin + first) * src.token_stride + head * src.head_stride;
-    const long long cell = (long long)where * p.cache.kv_heads + head;
-    int8_t* out = (blockIdx.z ? p.cache.v : p.cache.k) + cell * page * p.cache.d;
-    float* scale = (blockIdx.z ? p.cache.v_scales : p.cache.k_scales) + cell;
-    const float before = old ? *scale : 0.f;
-
-    // The largest magnitude, compared as bit patterns: those of non-negative
-    // floats order as the floats do, with infinity and NaN on top, so a NaN
-    // marks its page's scale instead of getting lost.
-    constexpr int KEEP = 4;
-    Raw8<T> kept[KEEP];
     // Item i is eights i % d8 of token i / d8; a thread's items are kThreads apart.
+    constexpr int KEEP = 4;
     const int step_row = kThreads / d8, step_col = kThreads % d8, row0 = threadIdx.x / d8, col0 = threadIdx.x % d8;
     auto next = [&](int& row, int& col) {
         row += step_row;
@@ -139,11 +119,27 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 8 : 7) cache_append
             ++row;
         }
     };
+    const int head = blockIdx.y;
+    const T* in = static_cast<const T*>(src.ptr) + (long long)(span.begin + first) * src.token_stride + head * src.head_stride;
+    const long long cell = (long long)where * p.cache.kv_heads + head;
+    int8_t* out = (blockIdx.z ? p.cache.v : p.cache.k) + cell * page * p.cache.d;
+    float* scale = (blockIdx.z ? p.cache.v_scales : p.cache.k_scales) + cell;
+    const float before = old ? *scale : 0.f;
+
+    // The largest magnitude, compared as bit patterns: those of non-negative
+    // floats order as the floats do, with infinity and NaN on top, so a NaN
+    // marks its page's scale instead of getting lost.
+    Pack<T, 8> kept[KEEP];
+    auto load = [&](Pack<T, 8>& x, int r, int c) {
+        const T* p8 = in + r * src.token_stride + c * 8;
+        if (vec) x.load(p8);
+        else x.load_some(p8, 8);
+    };
     uint32_t amax = 0;
     int row = row0, col = col0;
 #pragma unroll
     for (int n = 0; n < KEEP; ++n) {
-        if (row < fresh) kept[n].load(in + row * src.token_stride + col * 8, vec);
+        if (row < fresh) load(kept[n], row, col);
         next(row, col);
     }
     row = row0;
@@ -152,15 +148,15 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 8 : 7) cache_append
     for (int n = 0; n < KEEP; ++n) {
         if (row < fresh) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(kept[n][j]) & 0x7fffffffu);
+            for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(kept[n].get(j)) & 0x7fffffffu);
         }
         next(row, col);
     }
     for (int r = row, c = col; r < fresh; next(r, c)) {
-        Raw8<T> x;
-        x.load(in + r * src.token_stride + c * 8, vec);
+        Pack<T, 8> x;
+        load(x, r, c);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(x[j]) & 0x7fffffffu);
+        for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(x.get(j)) & 0x7fffffffu);
     }
     amax = __reduce_max_sync(0xffffffffu, amax);
     if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = amax;
@@ -188,11 +184,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 8 : 7) cache_append
         }
     }
     uint2* dst = reinterpret_cast<uint2*>(out + (long long)old * p.cache.d);
-    auto store = [&](int r, int c, const Raw8<T>& raw) {
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = raw[j];
-        dst[r * d8 + c] = round8(x, now, inv);
+    auto store = [&](int r, int c, const Pack<T, 8>& x) {
+        const uint2 u = inv != 0.f ? round8(x, now, inv) : round8_odd(in + r * src.token_stride + c * 8, now);
+        dst[r * d8 + c] = u;
     };
     row = row0;
     col = col0;
@@ -202,8 +196,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 8 : 7) cache_append
         next(row, col);
     }
     for (; row < fresh; next(row, col)) {
-        Raw8<T> x;
-        x.load(in + row * src.token_stride + col * 8, vec);
+        Pack<T, 8> x;
+        load(x, row, col);
         store(row, col, x);
     }
 }
@@ -285,6 +279,7 @@ cudaError_t launch_cache_append(const CacheAppendParams& p, cudaStream_t stream)
     if (p.total == 0 || p.table.sequences == 0) return cudaSuccess;
     const int esize = (int)dtype_size(p.dtype);
     const bool vec = vec8(p.k, esize) && vec8(p.v, esize);
+    // A sequence's ids are two more than the pages it fills.
     const dim3 grid((unsigned)(p.total / p.cache.page + 2ll * p.table.sequences), p.cache.kv_heads, 2);
     if (p.dtype == DT_F32) cache_append_kernel<float><<<grid, kThreads, 0, stream>>>(p, vec);
     else cache_append_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(p, vec);

@@ -15,15 +15,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <typename T, int VEC> struct VecType;
-template <> struct VecType<float, 4> { using type = uint4; };
-template <> struct VecType<float, 2> { using type = uint2; };
-template <> struct VecType<float, 1> { using type = uint32_t; };
-template <> struct VecType<__nv_bfloat16, 8> { using type = uint4; };
-template <> struct VecType<__nv_bfloat16, 4> { using type = uint2; };
-template <> struct VecType<__nv_bfloat16, 2> { using type = uint32_t; };
-template <> struct VecType<__nv_bfloat16, 1> { using type = uint16_t; };
-
 // The mask bits of columns [v, v + VEC) (v a multiple of VEC, so they lie in
 // one word), bit 0 first.
 __device__ __forceinline__ uint32_t mask_bits(const uint32_t* words, int v) { return __ldg(words + (v >> 5)) >> (v & 31); }
@@ -53,7 +44,6 @@ template <int VEC> constexpr int kRowCols = VEC == 8 ? 1 : 2;   // more would no
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, 5) logit_rules_rows_kernel(LogitRulesParams p) {
     constexpr int COLS = kRowCols<VEC>;
-    using V = typename VecType<T, VEC>::type;
     const int v0 = (blockIdx.x * kThreads * COLS + threadIdx.x) * VEC;
     float bias[COLS][VEC];
     uint32_t bits0[COLS];
@@ -66,7 +56,7 @@ __global__ void __launch_bounds__(kThreads, 5) logit_rules_rows_kernel(LogitRule
         for (int j = 0; j < VEC; ++j) bias[c][j] = p.bias && v + j < p.vocab ? __ldg(p.bias + v + j) : 0.f;
     }
     for (int r0 = blockIdx.y; r0 < p.rows; r0 += kRowsAhead * (int)gridDim.y) {
-        V x[kRowsAhead][COLS];
+        Pack<T, VEC> x[kRowsAhead][COLS];
         uint32_t bits[kRowsAhead][COLS];
 #pragma unroll
         for (int i = 0; i < kRowsAhead; ++i) {
@@ -78,14 +68,8 @@ __global__ void __launch_bounds__(kThreads, 5) logit_rules_rows_kernel(LogitRule
             for (int c = 0; c < COLS; ++c) {
                 const int v = v0 + c * kThreads * VEC;
                 bits[i][c] = shared ? bits0[c] : m && v < p.vocab ? mask_bits(m, v) : ~0u;
-                if (v + VEC <= p.vocab) {
-                    x[i][c] = __ldcs(reinterpret_cast<const V*>(in + v));
-                } else {
-                    T* e = reinterpret_cast<T*>(&x[i][c]);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j)
-                        if (v + j < p.vocab) e[j] = in[v + j];
-                }
+                if (v + VEC <= p.vocab) x[i][c].load(in + v);
+                else x[i][c].load_some(in + v, p.vocab - v);
             }
         }
 #pragma unroll
@@ -96,19 +80,10 @@ __global__ void __launch_bounds__(kThreads, 5) logit_rules_rows_kernel(LogitRule
 #pragma unroll
             for (int c = 0; c < COLS; ++c) {
                 const int v = v0 + c * kThreads * VEC;
-                T* e = reinterpret_cast<T*>(&x[i][c]);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float y = to_f(e[j]) + bias[c][j];
-                    e[j] = from_f<T>((bits[i][c] >> j) & 1u ? y : -INFINITY);
-                }
-                if (v + VEC <= p.vocab) {
-                    __stcs(reinterpret_cast<V*>(out + v), x[i][c]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j)
-                        if (v + j < p.vocab) out[v + j] = e[j];
-                }
+                for (int j = 0; j < VEC; ++j) x[i][c].put(j, (bits[i][c] >> j) & 1u ? x[i][c].get(j) + bias[c][j] : -INFINITY);
+                if (v + VEC <= p.vocab) x[i][c].store(out + v);
+                else x[i][c].store_some(out + v, p.vocab - v);
             }
         }
     }
@@ -120,21 +95,18 @@ constexpr int kRowThreads = 512, kAhead = 4;
 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kRowThreads) logit_rules_history_kernel(LogitRulesParams p, int chunk) {
-    using V = typename VecType<T, VEC>::type;
     extern __shared__ uint4 counts4[];
     uint32_t* counts = reinterpret_cast<uint32_t*>(counts4);
     const int row = blockIdx.y, lo = blockIdx.x * chunk, hi = min(lo + chunk, p.vocab);
     const T* in = static_cast<const T*>(p.logits) + row * p.ld;
     T* out = static_cast<T*>(p.out) + row * p.out_ld;
     auto load = [&](int v) {
-        V x;
-        if (v + VEC <= hi) return __ldcs(reinterpret_cast<const V*>(in + v));
-        T* e = reinterpret_cast<T*>(&x);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) e[j] = v + j < hi ? in[v + j] : from_f<T>(0.f);
+        Pack<T, VEC> x;
+        if (v + VEC <= hi) x.load(in + v);
+        else x.load_some(in + v, hi - v);
         return x;
     };
-    V ahead[kAhead];
+    Pack<T, VEC> ahead[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) ahead[i] = load(lo + (threadIdx.x + i * kRowThreads) * VEC);
     const Span h = seq_span(p.history_offsets, 0, row, p.history_total, p.status);
@@ -155,30 +127,36 @@ __global__ void __launch_bounds__(kRowThreads) logit_rules_history_kernel(LogitR
     const float freq = p.frequency ? p.frequency[row] : 0.f;
     const uint32_t* mask = mask_row(p, row);
     const bool bias4 = (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0;
-    auto apply = [&](int v, V x) {
+    auto apply = [&](int v, Pack<T, VEC> x) {
         const int live = min(VEC, hi - v);
-        T* e = reinterpret_cast<T*>(&x);
         const uint32_t bits = mask ? mask_bits(mask, v) : ~0u;
         // Bias and counts by fours where VEC has fours: a lane's neighbours are
         // VEC words on, so single words would meet in the same banks and sectors.
-        alignas(16) float bias[VEC];
-        alignas(16) uint32_t n[VEC];
-        constexpr int Q = VEC >= 4 ? VEC / 4 : 1;
+        float bias[VEC];
+        uint32_t n[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             bias[j] = 0.f;
             n[j] = 0;
         }
-        if (VEC >= 4 && live == VEC && bias4) {
-            if (p.bias) {
+        bool fours = false;
+        if constexpr (VEC >= 4) {
+            fours = live == VEC && bias4;
+            if (fours) {
 #pragma unroll
-                for (int q = 0; q < Q; ++q) *reinterpret_cast<float4*>(bias + 4 * q) = __ldg(reinterpret_cast<const float4*>(p.bias + v) + q);
+                for (int q = 0; q < VEC; q += 4) {
+                    if (p.bias) {
+                        const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + v + q));
+                        bias[q] = b.x; bias[q + 1] = b.y; bias[q + 2] = b.z; bias[q + 3] = b.w;
+                    }
+                    if (any) {
+                        const uint4 c = counts4[(v - lo + q) / 4];
+                        n[q] = c.x; n[q + 1] = c.y; n[q + 2] = c.z; n[q + 3] = c.w;
+                    }
+                }
             }
-            if (any) {
-#pragma unroll
-                for (int q = 0; q < Q; ++q) *reinterpret_cast<uint4*>(n + 4 * q) = counts4[(v - lo) / 4 + q];
-            }
-        } else {
+        }
+        if (!fours) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 if (j >= live) continue;
@@ -188,21 +166,15 @@ __global__ void __launch_bounds__(kRowThreads) logit_rules_history_kernel(LogitR
         }
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            float y = to_f(e[j]);
+            float y = x.get(j);
             if (n[j]) {
                 y = y > 0.f ? y / rep : y * rep;
                 y = y - freq * (float)n[j] - pres;
             }
-            y += bias[j];
-            e[j] = from_f<T>((bits >> j) & 1u ? y : -INFINITY);
+            x.put(j, (bits >> j) & 1u ? y + bias[j] : -INFINITY);
         }
-        if (live == VEC) {
-            __stcs(reinterpret_cast<V*>(out + v), x);
-        } else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (j < live) out[v + j] = e[j];
-        }
+        if (live == VEC) x.store(out + v);
+        else x.store_some(out + v, live);
     };
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {

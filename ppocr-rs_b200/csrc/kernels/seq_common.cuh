@@ -49,6 +49,67 @@ __device__ __forceinline__ int seq_offset(const int32_t* offsets, int uniform, i
     return offsets ? min(max(__ldg(offsets + i), 0), total) : i * uniform;
 }
 
+// VEC values of T as 32-bit words (a lone BF16 in the low half of one), read and
+// written 2, 4, 8 or 16 bytes at a time, 32 in two halves.  Words, so that they
+// stay in registers: an array of T seen through a pointer goes to local memory.
+template <typename T, int VEC>
+struct Pack {
+    static constexpr int kBytes = VEC * (int)sizeof(T), kWords = kBytes < 4 ? 1 : kBytes / 4;
+    uint32_t w[kWords];
+
+    __device__ __forceinline__ void load(const T* p) {   // aligned to its size (16 at most), streamed
+        if constexpr (kBytes >= 16) {
+#pragma unroll
+            for (int i = 0; i < kBytes / 16; ++i) {
+                const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+                w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+            }
+        } else if constexpr (kBytes == 8) {
+            const uint2 u = __ldcs(reinterpret_cast<const uint2*>(p));
+            w[0] = u.x; w[1] = u.y;
+        } else if constexpr (kBytes == 4) {
+            w[0] = __ldcs(reinterpret_cast<const uint32_t*>(p));
+        } else {
+            w[0] = __ldcs(reinterpret_cast<const uint16_t*>(p));
+        }
+    }
+    // The first `live` values one by one, zeros behind them.
+    __device__ __forceinline__ void load_some(const T* p, int live) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) put(j, j < live ? to_f(p[j]) : 0.f);
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (kBytes >= 16) {
+#pragma unroll
+            for (int i = 0; i < kBytes / 16; ++i)
+                __stcs(reinterpret_cast<uint4*>(p) + i, make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
+        } else if constexpr (kBytes == 8) {
+            __stcs(reinterpret_cast<uint2*>(p), make_uint2(w[0], w[1]));
+        } else if constexpr (kBytes == 4) {
+            __stcs(reinterpret_cast<uint32_t*>(p), w[0]);
+        } else {
+            __stcs(reinterpret_cast<uint16_t*>(p), (uint16_t)w[0]);
+        }
+    }
+    __device__ __forceinline__ void store_some(T* p, int live) const {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (j < live) p[j] = from_f<T>(get(j));
+    }
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+        else return __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+    }
+    __device__ __forceinline__ void put(int j, float x) {
+        if constexpr (sizeof(T) == 4) {
+            w[j] = __float_as_uint(x);
+        } else {
+            const uint32_t b = __bfloat16_as_ushort(__float2bfloat16_rn(x));
+            w[j / 2] = j & 1 ? __byte_perm(w[j / 2], b, 0x5410) : __byte_perm(b, w[j / 2], 0x7610);   // the other half stays
+        }
+    }
+};
+
 // 2^x by the hardware unit (relative error about 2^-22; 0 for -infinity).
 __device__ __forceinline__ float exp2_hw(float x) {
     float y;
