@@ -353,7 +353,7 @@ int ppocr_selftest_engine(ppocr_gpu* gpu, int planes, int n, int hi, int wi, int
  * arrive that never comes would in a forward.  kernel 0 = the BF16 tcgen05
  * GEMM, 1 = the engine with BF16 operands, 2 = the engine with FP32 operands
  * in three BF16 pieces, 3 = the split GEMM (FP32 activations split in shared
- * memory).  The kernel drains its copies and MMAs in flight,
+ * memory), 4 = the packed attention (its first block's second step).  The kernel drains its copies and MMAs in flight,
  * frees its TMEM and returns; the call then fails with PPOCR_ERR_GPU and
  * *code holds the kernel's wait-expiry code (nonzero).  The device stays
  * usable.  In a model forward the same expiry fails the forward with
@@ -590,7 +590,7 @@ int ppocr_gpu_synchronize(ppocr_gpu* gpu, void* stream, int timeout_ms);
  * A query that sees no key, or whose scores are all -infinity, gives zeros.
  * Masked keys and values never reach an output, whatever they hold.  Tokens of
  * `out` outside every sequence are left as they were.  d: 1..128; heads a
- * multiple of kv_heads; scale > 0 (0: d^-1/2).  The recognizers' encoder
+ * multiple of kv_heads; scale: 0 (d^-1/2) or positive, up to 1e30.  The recognizers' encoder
  * attention (src/cpu/model.rs:1705-1725) is the case of equal lengths. */
 typedef struct ppocr_attention_packed_args {
     int dtype;                   /* enum ppocr_dtype of q, k, v and out */

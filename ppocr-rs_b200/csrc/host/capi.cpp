@@ -354,7 +354,6 @@ void ppocr::gpu_release(ppocr_gpu* gpu) {
     if (gpu->side) cudaStreamDestroy(gpu->side);
     if (gpu->fork) cudaEventDestroy(gpu->fork);
     if (gpu->join) cudaEventDestroy(gpu->join);
-    PinnedFlags::release(gpu->seq_status);
     delete gpu;
 }
 
@@ -406,7 +405,6 @@ int ppocr_gpu_create(int device, ppocr_gpu** out) {
         cuda_check(cudaStreamCreateWithFlags(&g->side, cudaStreamNonBlocking), "create side stream");
         cuda_check(cudaEventCreateWithFlags(&g->fork, cudaEventDisableTiming), "create fork event");
         cuda_check(cudaEventCreateWithFlags(&g->join, cudaEventDisableTiming), "create join event");
-        static_assert(kSeqStatusWords <= (int)kFlags, "the status words come from the pinned flag sets");
         g->seq_status = PinnedFlags::acquire();
         std::fill_n(g->seq_status, kFlags, 0);
         *out = g.release();
@@ -1106,14 +1104,14 @@ int ppocr_model_profile(ppocr_model* model, size_t runs, double* op_ms) {
 int ppocr_selftest_wait_expiry(ppocr_gpu* gpu, int kernel, int wait_ms, int* code) {
     return guard([&] {
         if (!gpu || !code) fail(PPOCR_ERR_INVALID_INPUT, "null argument");
-        if (kernel < 0 || kernel > 3) fail(PPOCR_ERR_INVALID_INPUT, "invalid input: kernel must be 0..3");
+        if (kernel < 0 || kernel > 4) fail(PPOCR_ERR_INVALID_INPUT, "invalid input: kernel must be 0..4");
         if (wait_ms < 1 || wait_ms > 2000) fail(PPOCR_ERR_INVALID_INPUT, "invalid input: wait_ms outside 1..=2000");
         *code = 0;
         std::lock_guard<std::mutex> lock(gpu->mu);
         gpu->bind();
         // A 256 x 64 x 128 GEMM: two 128-row tiles, so CTA 1 runs normally while
         // CTA 0 waits for the first stage that its producer never loads.
-        const int m = 256, n = 64, k = 128, planes = kernel >= 2 ? 3 : 1;
+        const int m = 256, n = 64, k = 128, planes = kernel == 2 || kernel == 3 ? 3 : 1;
         ConvWeight cw;
         cw.cout = n; cw.cin = k; cw.kh = 1; cw.kw = 1;
         cw.w.assign((size_t)n * k, 0.5f);
@@ -1145,6 +1143,15 @@ int ppocr_selftest_wait_expiry(ppocr_gpu* gpu, int kernel, int wait_ms, int* cod
                 p.a = reinterpret_cast<const float*>(d + ao); p.w = d + wo; p.c = reinterpret_cast<float*>(d + co); p.ldc = n;
                 p.err = flag; p.wait_ns = limit; p.skip_load = 1;
                 e = launch_gemm_split(p, gpu->stream);
+            } else if (kernel == 4) {
+                // A as the queries, keys and values of 256 tokens of one head: two
+                // steps, of which the first block never gets the second's operands.
+                PackedAttentionParams p;
+                p.q = p.k = p.v = {d + ao, k, k};
+                p.out = {d + co, k, k};   // 256 x 128 BF16: as many bytes as C
+                p.sequences = 1; p.uniform = p.total_q = p.total_k = m; p.heads = p.kv_heads = 1; p.d = k; p.dtype = DT_BF16;
+                p.err = flag; p.wait_ns = limit; p.skip_load = 1;
+                e = launch_attention_tc(p, gpu->stream);
             } else {
                 TcEngineParams p;
                 p.mode = 0; p.planes = planes; p.m = m; p.n = n; p.k = k; p.n_pad = n_pad; p.k_pad = k_pad;
@@ -1719,6 +1726,9 @@ int ppocr_recognizer_forward_ctc_rules(ppocr_model* model, const float* input, s
         if (!model) fail(PPOCR_ERR_INVALID_INPUT, "model is null");
         if (model->m.kind != Kind::Recognizer) fail(PPOCR_ERR_INVALID_INPUT, "CTC decode needs a recognizer");
         const size_t classes = (size_t)model->m.classes, words = (classes + 31) / 32;
+        if (!input || input_len != model->input_elements())
+            fail(PPOCR_ERR_INVALID_INPUT, "input has " + std::to_string(input ? input_len : 0) + " values; expected " +
+                                              std::to_string(model->input_elements()));
         if (bias && !std::all_of(bias, bias + classes, [](float b) { return std::isfinite(b); }))
             fail(PPOCR_ERR_INVALID_INPUT, "invalid input: class biases must be finite");
         if (allowed) {

@@ -63,8 +63,10 @@ struct ppocr_gpu {
     size_t arena_bytes = 0;
     uint64_t arena_gen = 0;
     std::string name;
-    // What the sequence operators' kernels report (kSeqStatusWords ints of
-    // page-locked host memory that they write directly; see kernels/seq.h).
+    // What the sequence operators' kernels report, in page-locked host memory that
+    // they write directly: [0] 1 after a bad index, [1] the code of a pipeline
+    // wait that ran out.  Never given back: a captured graph may outlive the
+    // handle.
     int* seq_status = nullptr;
 
     void bind() const {

@@ -922,7 +922,7 @@ void svtr_head(Builder& b, const Act4& x, int cin, int hidden, int mlp) {
         ap.n = seq.n; ap.t = seq.h * seq.w; ap.heads = heads; ap.d = d; ap.scale = std::pow((float)d, -0.5f); ap.dtype = m.dtype;
         const int qt = qkv.tid, at = att.tid;
         m.plan.add_op(p + ".attention", {qt}, {at}, [ap, qt, at](const Ctx& c, cudaStream_t st) mutable {
-            ap.qkv = c.act(qt); ap.out = c.act(at);
+            ap.qkv = c.act(qt); ap.out = c.act(at); ap.err = c.err;
             return launch_attention(ap, st);
         }, "attention", 0, 4.0 * seq.n * heads * (double)ap.t * ap.t * d);
         GemmOpts op;

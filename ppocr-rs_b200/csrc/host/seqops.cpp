@@ -6,6 +6,7 @@
 #include <climits>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 
 #include "../kernels/seq.h"
@@ -74,13 +75,19 @@ void require_distinct(const ppocr_tokens& t, int64_t tokens, int heads, int d, c
     if (!token_major && !head_major) refuse(name, "'s strides make elements share memory");
 }
 
+// Counts leave room for a tile of tokens past the last one.
 int count_of(int64_t n, const char* what) {
-    require(n >= 0 && n <= INT_MAX, what);
+    require(n >= 0 && n < INT_MAX - 65536, what);
     return (int)n;
 }
 
+// Device arrays of 32-bit words (offsets, lengths, ids, floats).
+void require_words(std::initializer_list<const void*> arrays) {
+    for (const void* p : arrays) require(aligned(p, 4), "an array of 32-bit words is not aligned to them");
+}
+
 float scale_of(float scale, int d) {
-    require(std::isfinite(scale) && scale >= 0.f, "scale must be finite and not negative (0: d^-1/2)");
+    require(scale >= 0.f && scale <= 1e30f, "scale must be 0 (d^-1/2) or positive, up to 1e30");
     return scale == 0.f ? 1.f / std::sqrt((float)d) : scale;
 }
 
@@ -113,6 +120,7 @@ BlockTable table_of(const ppocr_block_table& t, const PagedCacheView& cache) {
     require(t.sequences >= 0 && t.width >= 0, "the block table's extents must not be negative");
     require(t.stride >= t.width || t.sequences <= 1, "the block table's stride is smaller than its width");
     require(t.pages || t.sequences == 0 || t.width == 0, "block table pointer is null");
+    require_words({t.pages});
     // Positions stay below 2^31 with room for a tile behind the last one.
     require((int64_t)t.width * cache.page <= INT_MAX - 4096, "the block table spans 2^31 tokens or more");
     require((int64_t)t.sequences * cache.kv_heads <= (1 << 30), "more than 2^30 sequences x heads");
@@ -157,10 +165,11 @@ int ppocr_attention_packed(ppocr_gpu* gpu, const ppocr_attention_packed_args* ar
         p.d = a.d;
         p.causal = a.causal;
         p.scale = scale_of(a.scale, a.d);
-        p.sequences = count_of(a.sequences, "sequences must be 0..2^31 - 1");
-        p.total_q = count_of(a.total_q, "total_q must be 0..2^31 - 1");
-        p.total_k = count_of(a.total_k, "total_k must be 0..2^31 - 1");
+        p.sequences = count_of(a.sequences, "sequences is negative or near 2^31");
+        p.total_q = count_of(a.total_q, "total_q is negative or near 2^31");
+        p.total_k = count_of(a.total_k, "total_k is negative or near 2^31");
         require(p.sequences == 0 || (a.q_offsets && a.k_offsets), "offsets pointer is null");
+        require_words({a.q_offsets, a.k_offsets});
         // The grid: one block per 64 rows of queries and group heads at most.
         require((int64_t)p.total_q * p.heads / 64 + ((int64_t)p.sequences + 1) * p.kv_heads <= INT_MAX,
                 "too many query rows for one call");
@@ -171,7 +180,8 @@ int ppocr_attention_packed(ppocr_gpu* gpu, const ppocr_attention_packed_args* ar
         require_distinct(a.out, a.total_q, a.heads, a.d, "out");
         p.q_offsets = a.q_offsets;
         p.k_offsets = a.k_offsets;
-        p.status = gpu->seq_status;
+        p.bad = gpu->seq_status;
+        p.err = gpu->seq_status + 1;
         OnDevice on(gpu);
         cuda_check(launch_attention_packed(p, stream_of(gpu, stream)), "packed attention");
     });
@@ -185,14 +195,15 @@ int ppocr_cache_append(ppocr_gpu* gpu, const ppocr_cache_append_args* args, void
         p.dtype = dtype_of(a.dtype);
         p.cache = cache_of(a.cache);
         p.table = table_of(a.table, p.cache);
-        p.total = count_of(a.total, "total must be 0..2^31 - 1");
+        p.total = count_of(a.total, "total is negative or near 2^31");
         require(p.table.sequences == 0 || (a.offsets && a.held), "offsets or held pointer is null");
+        require_words({a.offsets, a.held});
         require((int64_t)p.total / p.cache.page + 2 * (int64_t)p.table.sequences <= INT_MAX, "too many tokens for one call");
         p.k = tensor_of(a.k, a.total, p.dtype, "k");
         p.v = tensor_of(a.v, a.total, p.dtype, "v");
         p.offsets = a.offsets;
         p.held = a.held;
-        p.status = gpu->seq_status;
+        p.bad = gpu->seq_status;
         OnDevice on(gpu);
         cuda_check(launch_cache_append(p, stream_of(gpu, stream)), "cache append");
     });
@@ -206,15 +217,16 @@ int ppocr_cache_read(ppocr_gpu* gpu, const ppocr_cache_read_args* args, void* st
         p.dtype = dtype_of(a.dtype);
         p.cache = cache_of(a.cache);
         p.table = table_of(a.table, p.cache);
-        p.total = count_of(a.total, "total must be 0..2^31 - 1");
+        p.total = count_of(a.total, "total is negative or near 2^31");
         require(p.table.sequences == 0 || (a.offsets && a.first), "offsets or first pointer is null");
+        require_words({a.offsets, a.first});
         p.k = tensor_of(a.k, a.total, p.dtype, "k");
         p.v = tensor_of(a.v, a.total, p.dtype, "v");
         require_distinct(a.k, a.total, p.cache.kv_heads, p.cache.d, "k");
         require_distinct(a.v, a.total, p.cache.kv_heads, p.cache.d, "v");
         p.offsets = a.offsets;
         p.first = a.first;
-        p.status = gpu->seq_status;
+        p.bad = gpu->seq_status;
         OnDevice on(gpu);
         cuda_check(launch_cache_read(p, stream_of(gpu, stream)), "cache read");
     });
@@ -234,11 +246,12 @@ int ppocr_attention_cached(ppocr_gpu* gpu, const ppocr_attention_cached_args* ar
         p.heads = a.heads;
         p.scale = scale_of(a.scale, p.cache.d);
         require(p.table.sequences == 0 || a.lengths, "lengths pointer is null");
+        require_words({a.lengths});
         p.q = tensor_of(a.q, p.table.sequences, p.dtype, "q");
         p.out = tensor_of(a.out, p.table.sequences, p.dtype, "out");
         require_distinct(a.out, p.table.sequences, a.heads, p.cache.d, "out");
         p.lengths = a.lengths;
-        p.status = gpu->seq_status;
+        p.bad = gpu->seq_status;
         OnDevice on(gpu);
         cuda_check(launch_attention_cached(p, stream_of(gpu, stream)), "cached attention");
     });
@@ -259,11 +272,12 @@ int ppocr_logit_rules(ppocr_gpu* gpu, const ppocr_logit_rules_args* args, void* 
                 "a row stride is negative or beyond 2^40");
         require(a.logits != a.out || a.rows <= 1 || a.stride == a.out_stride, "in place, both row strides must be the same");
         require(!(a.repetition || a.presence || a.frequency) || a.history_offsets, "the penalties need a history");
-        p.history_total = count_of(a.history_total, "history_total must be 0..2^31 - 1");
+        p.history_total = count_of(a.history_total, "history_total is negative or near 2^31");
         require(!a.history_offsets || a.history || p.history_total == 0, "history pointer is null");
         require(!a.mask_index || a.mask, "mask_index needs a mask");
         require(!a.mask || (a.states >= 1 && a.mask_stride >= ((int64_t)a.vocab + 31) / 32),
                 "a mask needs at least one row of ceil(vocab / 32) words");
+        require_words({a.history, a.history_offsets, a.repetition, a.presence, a.frequency, a.bias, a.mask, a.mask_index});
         p.logits = a.logits;
         p.out = a.out;
         p.ld = a.stride;
@@ -280,7 +294,7 @@ int ppocr_logit_rules(ppocr_gpu* gpu, const ppocr_logit_rules_args* args, void* 
         p.mask_ld = a.mask_stride;
         p.states = a.states;
         p.mask_index = a.mask_index;
-        p.status = gpu->seq_status;
+        p.bad = gpu->seq_status;
         OnDevice on(gpu);
         cuda_check(launch_logit_rules(p, stream_of(gpu, stream)), "logit rules");
     });

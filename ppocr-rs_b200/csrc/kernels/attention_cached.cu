@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
     int len = p.lengths[seq];
     const long long room = (long long)p.table.width * page;
     if (len < 0 || len > room) {
-        if (threadIdx.x == 0) seq_bad_index(p.status);
+        if (threadIdx.x == 0) seq_bad_index(p.bad);
         len = len < 0 ? 0 : (int)room;
     }
     // Pairs of tiles, dealt to the splits in ranges and to a block's warps by turns.
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
         if (pair >= t_end || tile >= tiles) return -1;
         const int w = __ldg(pages + (tile >> page_shift));
         if ((unsigned)w >= (unsigned)p.cache.pages) {
-            seq_bad_index(p.status);
+            seq_bad_index(p.bad);
             return -1;
         }
         return w;

@@ -105,8 +105,8 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 5) atten
         return (long long)seq_offset(p.q_offsets, p.uniform, i, p.total_q) * group / kRows + i;
     };
     const int seq = find_owner(p.sequences, id, first_id);
-    const Span qs = seq_span(p.q_offsets, p.uniform, seq, p.total_q, p.status);
-    const Span ks = seq_span(p.k_offsets, p.uniform, seq, p.total_k, p.status);
+    const Span qs = seq_span(p.q_offsets, p.uniform, seq, p.total_q, p.bad);
+    const Span ks = seq_span(p.k_offsets, p.uniform, seq, p.total_k, p.bad);
     const long long row0 = (id - first_id(seq)) * kRows, all = (long long)qs.len * group;
     if (row0 < 0 || row0 >= all) return;
     const int rows = (int)min((long long)kRows, all - row0);
@@ -393,7 +393,13 @@ cudaError_t launch_type(const PackedAttentionParams& p, cudaStream_t stream) {
 
 cudaError_t launch_attention_packed(const PackedAttentionParams& p, cudaStream_t stream) {
     if (p.total_q == 0 || p.sequences == 0) return cudaSuccess;
-    if ((long long)p.total_k >= 256ll * p.sequences && attention_tc_supported(p)) return launch_attention_tc(p, stream);
+    // tcgen05 from 16,384 keys x (padded) values per sequence on.  Measured on
+    // 16,384 tokens in causal sequences of equal length, mma.sync / tcgen05 in us:
+    //   8 heads of 24          length 384: 44 / 57, 512: 53 / 55, 1,024: 89 / 67
+    //   16 of 64, 4 KV heads   length 128: 62 / 72, 192: 72 / 73, 256: 83 / 74
+    //   8 of 128               length 96: 95 / 83, 128: 82 / 68, 512: 150 / 64
+    const int padded = p.d <= 16 ? 16 : p.d <= 32 ? 32 : p.d <= 64 ? 64 : 128;
+    if ((long long)p.total_k * padded >= 16384ll * p.sequences && attention_tc_supported(p)) return launch_attention_tc(p, stream);
     return p.dtype == DT_F32 ? launch_type<float>(p, stream) : launch_type<__nv_bfloat16>(p, stream);
 }
 

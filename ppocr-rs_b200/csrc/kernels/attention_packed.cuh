@@ -50,9 +50,4 @@ inline bool rows16(const SeqTensor& t, int esize) {
     return ((reinterpret_cast<uintptr_t>(t.ptr) | (uintptr_t)(t.token_stride * esize) | (uintptr_t)(t.head_stride * esize)) & 15) == 0;
 }
 
-// tcgen05 kernel (attention_tc.cu): BF16, 16-byte aligned rows, d a multiple
-// of 8 and at most 128 query heads to a KV head.
-bool attention_tc_supported(const PackedAttentionParams& p);
-cudaError_t launch_attention_tc(const PackedAttentionParams& p, cudaStream_t stream);
-
 }  // namespace ppocr

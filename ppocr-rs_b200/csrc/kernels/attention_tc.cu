@@ -18,7 +18,7 @@
 // passes it by more than 8 (in log2: weights up to 2^8), so the output
 // accumulator in TMEM is rarely rescaled.
 //
-// Every wait is bounded: on expiry the CTA records a code in status[1], stops,
+// Every wait is bounded: on expiry the CTA records a code in *err, stops,
 // lets its copies and MMAs land, frees its TMEM and returns.  Rows that come
 // out non-finite are computed again from their definition (attend_row).
 #include <cuda.h>
@@ -127,7 +127,7 @@ __device__ __forceinline__ bool elect_one() {
 
 // tc::mbar_wait without its first read of the global timer, which takes longer
 // than most waits here: the timer is read once in 4,096 tries.
-__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, const volatile int* abort) {
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, const volatile int* abort, uint64_t limit_ns) {
     const uint32_t addr = tc::smem_u32(bar);
     uint64_t start = 0;
     for (uint32_t i = 1;; ++i) {
@@ -144,7 +144,7 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, const
         if ((i & 4095) == 0) {
             const uint64_t now = tc::globaltimer_ns();
             if (start == 0) start = now;
-            else if (now - start > tc::kWaitNs) return false;
+            else if (now - start > limit_ns) return false;
         }
     }
 }
@@ -172,8 +172,8 @@ __device__ __forceinline__ bool find_work(const PackedAttentionParams& p, Work& 
     const int id = p.causal ? pieces - 1 - at : at;   // the longest rows first
     auto first_id = [&](int i) { return seq_offset(p.q_offsets, p.uniform, i, p.total_q) / step + i; };
     w.seq = find_owner(p.sequences, id, first_id);
-    w.qs = seq_span(p.q_offsets, p.uniform, w.seq, p.total_q, p.status);
-    w.ks = seq_span(p.k_offsets, p.uniform, w.seq, p.total_k, p.status);
+    w.qs = seq_span(p.q_offsets, p.uniform, w.seq, p.total_q, p.bad);
+    w.ks = seq_span(p.k_offsets, p.uniform, w.seq, p.total_k, p.bad);
     const int index = id - first_id(w.seq);
     if (index < 0 || index > w.qs.len / step) return false;
     w.token0 = index * step;
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     const uint32_t tmem = tmem_slot;
     const uint32_t tm_s[kTiles] = {tmem, tmem + kKeys}, tm_o[kTiles] = {tmem + 2 * kKeys, tmem + 2 * kKeys + 64 * DC};
     auto expired = [&](int code) {
-        if (p.status) reinterpret_cast<volatile int*>(p.status)[1] = code;
+        if (p.err) *reinterpret_cast<volatile int*>(p.err) = code;
         abort_flag = 1;
     };
 
@@ -260,16 +260,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         if (warp == kSoftmaxWarps && steps > 0) {
             int i = 1;
             for (; i <= steps; ++i) {
-                if (i >= L::stages && !__all_sync(0xffffffffu, wait_phase(&empty[i % L::stages], (i / L::stages + 1) & 1, &abort_flag))) {
+                if (i >= L::stages && !__all_sync(0xffffffffu, wait_phase(&empty[i % L::stages], (i / L::stages + 1) & 1, &abort_flag, p.wait_ns))) {
                     expired(1);
                     break;
                 }
-                if (elect_one()) load_stage(i);
+                const bool skip = p.skip_load && i == 1 && blockIdx.x == 0;
+                if (!skip && elect_one()) load_stage(i);
                 __syncwarp();
             }
             // No copy is in flight when the CTA ends, however it ends.
-            tc::mbar_wait(&q_full, 0, false);
-            for (int b = max(0, i - L::stages); b < i; ++b) tc::mbar_wait(&full[b % L::stages], (b / L::stages) & 1, false);
+            tc::mbar_wait(&q_full, 0, false, p.wait_ns);
+            for (int b = max(0, i - L::stages); b < i; ++b) tc::mbar_wait(&full[b % L::stages], (b / L::stages) & 1, false, p.wait_ns);
         } else if (warp == kSoftmaxWarps + 1 && steps > 0) {
             // An issued instruction costs this warp 30 to 50 cycles and a wait 200
             // although its phase is long complete, so there are as few as can be:
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             const uint32_t v_desc = desc_low(tc::smem_u32(ring), kChunk);
             bool ok = true;
             auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-                if (ok && !__all_sync(0xffffffffu, wait_phase(bar, parity, &abort_flag))) {
+                if (ok && !__all_sync(0xffffffffu, wait_phase(bar, parity, &abort_flag, p.wait_ns))) {
                     expired(code);
                     ok = false;
                 }
@@ -342,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             // Every MMA this warp issued completes before TMEM is freed.
             if (elect_one()) tc::commit(&drain);
             __syncwarp();
-            tc::mbar_wait(&drain, 0, false);
+            tc::mbar_wait(&drain, 0, false, tc::kWaitNs);
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -357,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         float top = -INFINITY, ref = 0.f, sum = 0.f;   // ref: top, 0 while it is -infinity
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-            ok = __all_sync(0xffffffffu, wait_phase(bar, parity, &abort_flag));
+            ok = __all_sync(0xffffffffu, wait_phase(bar, parity, &abort_flag, p.wait_ns));
             if (!ok) expired(code);
             tc::fence_after();
         };
@@ -512,6 +513,8 @@ bool mappable(const SeqTensor& t, int heads, int tokens) {
 template <int DC>
 cudaError_t launch_dc(const PackedAttentionParams& p, cudaStream_t stream) {
     const int group = p.heads / p.kv_heads, per = kRows / group;
+    PackedAttentionParams a = p;
+    if (!a.wait_ns) a.wait_ns = tc::kWaitNs;
     CUtensorMap mq, mk, mv;
     if (!make_map(&mq, p.q, p.d, p.heads, p.total_q, group, per) || !make_map(&mk, p.k, p.d, p.kv_heads, p.total_k, 1, kKeys) ||
         !make_map(&mv, p.v, p.d, p.kv_heads, p.total_k, 1, kKeys))
@@ -519,7 +522,7 @@ cudaError_t launch_dc(const PackedAttentionParams& p, cudaStream_t stream) {
     cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(attention_tc_kernel<DC>), Layout<DC>::smem);
     if (e != cudaSuccess) return e;
     const long long pieces = (long long)p.total_q / (kTiles * per) + p.sequences;
-    attention_tc_kernel<DC><<<(unsigned)(pieces * p.kv_heads), kThreads, Layout<DC>::smem, stream>>>(mq, mk, mv, p, rows16(p.out, 2));
+    attention_tc_kernel<DC><<<(unsigned)(pieces * p.kv_heads), kThreads, Layout<DC>::smem, stream>>>(mq, mk, mv, a, rows16(p.out, 2));
     return cudaGetLastError();
 }
 

@@ -407,6 +407,7 @@ struct AttentionParams {
     void* out = nullptr;
     float scale = 1.f;
     DType dtype = DT_F32;
+    int* err = nullptr;                  // as GemmParams::err (long lines take the packed attention)
 };
 cudaError_t launch_attention(const AttentionParams& p, cudaStream_t stream);
 

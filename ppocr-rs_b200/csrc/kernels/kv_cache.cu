@@ -90,11 +90,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 8 : 7) cache_append
     auto first_id = [&](int i) { return (seq_offset(p.offsets, 0, i, p.total) >> page_shift) + 2 * i; };
     const int seq = find_owner(p.table.sequences, id, first_id);
     const int index = id - first_id(seq);   // of the pages this sequence's new tokens touch
-    const Span span = seq_span(p.offsets, 0, seq, p.total, p.status);
+    const Span span = seq_span(p.offsets, 0, seq, p.total, p.bad);
     const int held = p.held[seq];
     if (span.len == 0 || index < 0) return;
     if (held < 0 || (long long)held + span.len > (long long)p.table.width * page) {
-        if (threadIdx.x == 0) seq_bad_index(p.status);
+        if (threadIdx.x == 0) seq_bad_index(p.bad);
         return;
     }
     const int old = index == 0 ? held % page : 0;                      // slots filled before
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 8 : 7) cache_append
     const int block = held / page + index;
     const int where = p.table.pages[seq * p.table.stride + block];
     if (where < 0 || where >= p.cache.pages) {
-        if (threadIdx.x == 0) seq_bad_index(p.status);
+        if (threadIdx.x == 0) seq_bad_index(p.bad);
         return;
     }
     const SeqTensor& src = blockIdx.z ? p.v : p.k;
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kReadThreads) cache_read_kernel(CacheReadParam
             }
             if (w < 0 || w >= p.cache.pages) {
                 w = -1;
-                if (lane == 0) seq_bad_index(p.status);
+                if (lane == 0) seq_bad_index(p.bad);
             }
         }
         if (lane == 0) {

@@ -24,11 +24,11 @@ __device__ __forceinline__ const uint32_t* mask_row(const LogitRulesParams& p, i
     if (!p.mask) return nullptr;
     const int state = p.mask_index ? p.mask_index[row] : 0;
     if (state < 0) {
-        if (state != -1) seq_bad_index(p.status);
+        if (state != -1) seq_bad_index(p.bad);
         return nullptr;
     }
     if (state >= p.states) {
-        seq_bad_index(p.status);
+        seq_bad_index(p.bad);
         return nullptr;
     }
     return p.mask + (long long)state * p.mask_ld;
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(kRowThreads) logit_rules_history_kernel(LogitR
     Pack<T, VEC> ahead[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) ahead[i] = load(lo + (threadIdx.x + i * kRowThreads) * VEC);
-    const Span h = seq_span(p.history_offsets, 0, row, p.history_total, p.status);
+    const Span h = seq_span(p.history_offsets, 0, row, p.history_total, p.bad);
     const bool any = h.len > 0;
     if (any) {
         for (int i = threadIdx.x; i < (hi - lo + 3) / 4; i += kRowThreads) counts4[i] = make_uint4(0, 0, 0, 0);
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kRowThreads) logit_rules_history_kernel(LogitR
         for (int i = threadIdx.x; i < h.len; i += kRowThreads) {
             const int id = __ldg(p.history + h.begin + i);
             if (id >= lo && id < hi) atomicAdd(&counts[id - lo], 1u);
-            else if (id < 0 || id >= p.vocab) seq_bad_index(p.status);
+            else if (id < 0 || id >= p.vocab) seq_bad_index(p.bad);
         }
         __syncthreads();
     }

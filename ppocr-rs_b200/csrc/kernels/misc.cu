@@ -859,6 +859,7 @@ cudaError_t launch_attention(const AttentionParams& p, cudaStream_t stream) {
         a.d = p.d;
         a.scale = p.scale;
         a.dtype = p.dtype;
+        a.err = p.err;
         return launch_attention_packed(a, stream);
     }
     {

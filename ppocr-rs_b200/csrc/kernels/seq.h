@@ -7,8 +7,8 @@
 // Strides are in elements; the last axis of every tensor is contiguous.
 // Offsets, lengths and block tables live on the device.  The kernels clamp
 // them to the tensors' extents, so a bad one reads and writes nothing out of
-// bounds, and store SEQ_BAD_INDEX in *status (host memory mapped into the
-// device's address space) for the host to raise.
+// bounds, and set *bad to 1 (for the C ABI page-locked host memory, which the
+// host reads and raises; null: not reported).
 #pragma once
 
 #include <cuda_runtime.h>
@@ -17,10 +17,6 @@
 #include "kernels.h"
 
 namespace ppocr {
-
-enum SeqStatus : int { SEQ_OK = 0, SEQ_BAD_INDEX = 1 };
-// status[0] holds a SeqStatus, status[1] the code of a pipeline wait that ran out.
-constexpr int kSeqStatusWords = 2;
 
 struct SeqTensor {
     void* ptr = nullptr;
@@ -39,10 +35,21 @@ struct PackedAttentionParams {
     int causal = 0;
     float scale = 1.f;                   // > 0
     DType dtype = DT_F32;
-    int* status = nullptr;               // may be null
+    int* bad = nullptr;
+    // tcgen05 kernel: a pipeline wait that runs out stores its code in *err (null:
+    // not reported) after wait_ns (0: 2 s); skip_load = 1 (self-test only) leaves
+    // block 0's second stage unloaded so that the waits on it run out.
+    int* err = nullptr;
+    uint64_t wait_ns = 0;
+    int skip_load = 0;
 };
 constexpr int kPackedMaxD = 128;
 cudaError_t launch_attention_packed(const PackedAttentionParams& p, cudaStream_t stream);
+
+// Its tcgen05 kernel (attention_tc.cu): BF16, 16-byte aligned rows, d a multiple
+// of 8 and at most 128 query heads to a KV head.
+bool attention_tc_supported(const PackedAttentionParams& p);
+cudaError_t launch_attention_tc(const PackedAttentionParams& p, cudaStream_t stream);
 
 // 8-bit cache: values[page][head][slot][d] with one FP32 scale per (page, head).
 struct PagedCacheView {
@@ -67,7 +74,7 @@ struct CacheAppendParams {
     const int32_t* held = nullptr;       // [sequences] tokens already in the cache
     int total = 0;
     DType dtype = DT_F32;
-    int* status = nullptr;
+    int* bad = nullptr;
 };
 cudaError_t launch_cache_append(const CacheAppendParams& p, cudaStream_t stream);
 
@@ -79,7 +86,7 @@ struct CacheReadParams {
     const int32_t* first = nullptr;      // [sequences] position of each sequence's first token read
     int total = 0;
     DType dtype = DT_F32;
-    int* status = nullptr;
+    int* bad = nullptr;
 };
 cudaError_t launch_cache_read(const CacheReadParams& p, cudaStream_t stream);
 
@@ -91,7 +98,7 @@ struct CachedAttentionParams {
     int heads = 0;
     float scale = 1.f;                   // > 0
     DType dtype = DT_F32;
-    int* status = nullptr;
+    int* bad = nullptr;
 };
 cudaError_t launch_attention_cached(const CachedAttentionParams& p, cudaStream_t stream);
 
@@ -115,7 +122,7 @@ struct LogitRulesParams {
     int states = 0;
     const int32_t* mask_index = nullptr; // [rows] state of each row, -1: unmasked; null: state 0 for all
     DType dtype = DT_F32;
-    int* status = nullptr;
+    int* bad = nullptr;
 };
 cudaError_t launch_logit_rules(const LogitRulesParams& p, cudaStream_t stream);
 

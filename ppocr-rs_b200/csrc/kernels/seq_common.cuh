@@ -7,8 +7,8 @@
 
 namespace ppocr {
 
-__device__ __forceinline__ void seq_bad_index(int* status) {
-    if (status) *reinterpret_cast<volatile int*>(status) = SEQ_BAD_INDEX;
+__device__ __forceinline__ void seq_bad_index(int* bad) {
+    if (bad) *reinterpret_cast<volatile int*>(bad) = 1;
 }
 
 struct Span {
@@ -17,10 +17,10 @@ struct Span {
 
 // Tokens [begin, begin + len) of sequence i, clamped to [0, total); a negative,
 // decreasing or too large offset is reported.
-__device__ __forceinline__ Span seq_span(const int32_t* offsets, int uniform, int i, int total, int* status) {
+__device__ __forceinline__ Span seq_span(const int32_t* offsets, int uniform, int i, int total, int* bad) {
     if (!offsets) return Span{i * uniform, uniform};
     const int b = offsets[i], e = offsets[i + 1];
-    if (b < 0 || e < b || e > total) seq_bad_index(status);
+    if (b < 0 || e < b || e > total) seq_bad_index(bad);
     const int cb = min(max(b, 0), total);
     return Span{cb, min(max(e, cb), total) - cb};
 }

@@ -503,7 +503,7 @@ class Gpu:
 
     def selftest_wait_expiry(self, kernel: int, wait_ms: int = 20) -> int:
         """Makes one tensor-core pipeline wait run out (kernel 0: BF16 GEMM, 1 / 2:
-        the engine with 1 / 3 operand planes); raises GpuError carrying the
+        the engine with 1 / 3 operand planes, 3: the split GEMM, 4: the packed attention); raises GpuError carrying the
         kernel's wait-expiry code as `.wait_code`."""
         code = C.c_int()
         status = library().ppocr_selftest_wait_expiry(self._h, int(kernel), int(wait_ms), C.byref(code))

@@ -258,6 +258,15 @@ def test_packed_bad_offsets_are_reported_and_stay_in_bounds(gpu):
     gpu.synchronize(s)   # reported once
 
 
+def test_packed_wait_expiry_fails_cleanly(gpu):
+    """The tcgen05 kernel's waits are bounded: a block whose second step never arrives gives up, and the device
+    still computes."""
+    with pytest.raises(P.GpuError, match="wait ran out") as info:
+        gpu.selftest_wait_expiry(4, 20)
+    assert info.value.wait_code != 0
+    run_packed(gpu, [600, 700], [600, 700], 4, 2, 128, "bf16", True)
+
+
 def test_packed_nothing_to_do(gpu):
     s = torch.cuda.current_stream()
     e = torch.empty(0, 2, 16, device="cuda")

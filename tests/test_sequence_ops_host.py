@@ -159,6 +159,43 @@ def test_other_refusals(gpu, call, change, words):
         call(gpu, **change)
 
 
+@pytest.mark.parametrize("call,change", [
+    (packed, dict(q_offsets=arr((3,), "i32", ptr=A + 2))), (packed, dict(k_offsets=arr((3,), "i32", ptr=A + 1))),
+    (cached, dict(lengths=arr((3,), "i32", ptr=A + 2))), (cached, dict(table=arr((3, 2), "i32", ptr=A + 2))),
+    (append, dict(offsets=arr((4,), "i32", ptr=A + 1))), (append, dict(held=arr((3,), "i32", ptr=A + 2))),
+    (read, dict(first=arr((3,), "i32", ptr=A + 2))), (rules, dict(bias=arr((100,), ptr=A + 2))),
+    (rules, dict(mask=arr((1, 4), "i32", ptr=A + 2))),
+    (rules, dict(mask=arr((1, 4), "i32"), mask_index=arr((4,), "i32", ptr=A + 1))),
+    (rules, dict(history=arr((7,), "i32", ptr=A + 2), history_offsets=arr((5,), "i32"))),
+    (rules, dict(history=arr((7,), "i32"), history_offsets=arr((5,), "i32", ptr=A + 2))),
+    (rules, dict(history=arr((7,), "i32"), history_offsets=arr((5,), "i32"), repetition=arr((4,), ptr=A + 2))),
+])
+def test_misaligned_arrays_are_refused(gpu, call, change):
+    with pytest.raises(P.InvalidInput, match="aligned"):
+        call(gpu, **change)
+
+
+def test_argument_layouts_are_the_headers(tmp_path):
+    """The packed arguments have the sizes and ends of the header's structures."""
+    import os
+    import shutil
+    import subprocess
+
+    if shutil.which("g++") is None:
+        pytest.skip("needs a C++ compiler")
+    ends = [("ppocr_attention_packed_args", "k_offsets"), ("ppocr_cache_append_args", "held"), ("ppocr_cache_read_args", "first"),
+            ("ppocr_attention_cached_args", "lengths"), ("ppocr_logit_rules_args", "mask_index")]
+    src = tmp_path / "layout.cpp"
+    src.write_text('#include "ppocr_b200.h"\n#include <cstdio>\nint main() {\n' + "".join(
+        f'std::printf("%zu %zu\\n", sizeof({t}), offsetof({t}, {m}));\n' for t, m in ends) + "}\n")
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["g++", "-I", include, str(src), "-o", str(tmp_path / "layout")], check=True)
+    out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split("\n")
+    for line, pack in zip(out, (P._ATTENTION_PACKED, P._CACHE_TOKENS, P._CACHE_TOKENS, P._ATTENTION_CACHED, P._LOGIT_RULES)):
+        size, last = (int(v) for v in line.split())
+        assert pack.__self__.size == size == last + 8
+
+
 def test_null_handles_and_arguments():
     lib = P.library()
     for name in ("ppocr_attention_packed", "ppocr_cache_append", "ppocr_cache_read", "ppocr_attention_cached",
