@@ -644,13 +644,15 @@ class Gpu:
 
     def _paged(self, cache: PagedCache, table):
         """The cache's and the table's fields, the cache's heads and d, and the table's sequences."""
-        dev, shape = self.device, _shape(cache.k, "cache.k", 4)
-        t = _shape(table, "table", 2)
-        fields = (_flat(cache.k, "cache.k", "i8", shape, dev), _flat(cache.v, "cache.v", "i8", shape, dev),
-                  _flat(cache.k_scales, "cache.k_scales", "f32", shape[:2], dev),
-                  _flat(cache.v_scales, "cache.v_scales", "f32", shape[:2], dev), *shape,
+        dev, k = self.device, cache.k
+        shape, t = _shape(k, "cache.k", 4), _shape(table, "table", 2)
+        pages, heads, page, d = shape
+        scales = (pages, heads)
+        fields = (_flat(k, "cache.k", "i8", shape, dev), _flat(cache.v, "cache.v", "i8", shape, dev),
+                  _flat(cache.k_scales, "cache.k_scales", "f32", scales, dev),
+                  _flat(cache.v_scales, "cache.v_scales", "f32", scales, dev), pages, heads, page, d,
                   *_rows(table, "table", "i32", t, dev), *t)
-        return fields, shape[1], shape[3], t[0]
+        return fields, heads, d, t[0]
 
     def _cache_tokens(self, call, cache, k, v, offsets, positions, what, table, stream):
         dev = self.device
