@@ -45,6 +45,77 @@ __device__ __noinline__ void attend_row(const T* q, const T* k, long long k_stri
         if (lane + 32 * i < d) out[lane + 32 * i] = from_f<T>(nan ? NAN : sum == 0.f ? 0.f : acc[i] / sum);
 }
 
+// A block's piece of the mma.sync kernels: up to ROWS rows (row = query token x
+// group + head) of one (sequence, KV head).
+template <int ROWS>
+struct PackedPiece {
+    Span qs, ks;
+    int kv, group, rows;       // rows <= 0: nothing to do
+    int token0, part0, shift;  // row n is query token0 + (part0 + n) / group; causal: query i sees keys j <= i + shift
+    bool causal;
+
+    __device__ __forceinline__ explicit PackedPiece(const PackedAttentionParams& p) {
+        group = p.heads / p.kv_heads;
+        kv = blockIdx.x % p.kv_heads;
+        causal = p.causal;
+        // The longest rows of a causal sequence are dealt first.
+        const long long pieces = gridDim.x / p.kv_heads, at_id = blockIdx.x / p.kv_heads;
+        const long long id = causal ? pieces - 1 - at_id : at_id;
+        auto first_id = [&](int i) { return (long long)seq_offset(p.q_offsets, p.uniform, i, p.total_q) * group / ROWS + i; };
+        const int seq = find_owner(p.sequences, id, first_id);
+        qs = seq_span(p.q_offsets, p.uniform, seq, p.total_q, p.bad);
+        ks = seq_span(p.k_offsets, p.uniform, seq, p.total_k, p.bad);
+        const long long row0 = (id - first_id(seq)) * ROWS, all = (long long)qs.len * group;
+        rows = row0 < 0 ? 0 : (int)max(min((long long)ROWS, all - row0), 0ll);
+        shift = ks.len - qs.len;
+        token0 = (int)(row0 / group);
+        part0 = (int)(row0 % group);
+    }
+    __device__ __forceinline__ int keys_of(int n) const {
+        return causal ? min(max(token0 + (part0 + n) / group + shift + 1, 0), ks.len) : ks.len;
+    }
+    template <typename T>
+    __device__ __forceinline__ T* queries(const SeqTensor& t) const {
+        return static_cast<T*>(t.ptr) + (qs.begin + (long long)token0) * t.token_stride + (long long)kv * group * t.head_stride;
+    }
+    template <typename T>
+    __device__ __forceinline__ const T* keys(const SeqTensor& t) const {
+        return static_cast<const T*>(t.ptr) + (long long)ks.begin * t.token_stride + kv * t.head_stride;
+    }
+    __device__ __forceinline__ long long row_at(const SeqTensor& t, int n) const {
+        const int x = part0 + n;
+        return (long long)(x / group) * t.token_stride + (x % group) * t.head_stride;
+    }
+    // Blocks of a launch: sequence i owns the ids from floor(offset_i group / ROWS) + i, at least its number of pieces.
+    static long long blocks(const PackedAttentionParams& p) {
+        return ((long long)p.total_q * (p.heads / p.kv_heads) / ROWS + p.sequences) * p.kv_heads;
+    }
+};
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool live) {
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"((uint32_t)__cvta_generic_to_shared(p)));
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"((uint32_t)__cvta_generic_to_shared(p)));
+}
+
+// Whether pairs of a tensor's values are aligned to their size.
+inline bool pairs_aligned(const SeqTensor& t, int esize) {
+    return ((reinterpret_cast<uintptr_t>(t.ptr) | (uintptr_t)(t.token_stride * esize) | (uintptr_t)(t.head_stride * esize)) %
+            (2 * esize)) == 0;
+}
+
 // Whether every row of a tensor starts on a 16-byte boundary.
 inline bool rows16(const SeqTensor& t, int esize) {
     return ((reinterpret_cast<uintptr_t>(t.ptr) | (uintptr_t)(t.token_stride * esize) | (uintptr_t)(t.head_stride * esize)) & 15) == 0;

@@ -1,0 +1,390 @@
+// Attention over packed sequences in FP32, on mma.sync m16n8k16 with FP16
+// operands: every head size up to 128, stride and length.
+//
+// Every value is carried as two FP16 pieces (22 bits) of the value times a
+// power of two, and a product as its three leading ones: FP32-class, at half
+// the tensor-core time of TF32 pieces (whose MMAs hold half the values).  FP16's
+// range is met by one power of two per row of Q, K and V, the one that takes the
+// row's largest magnitude into [2^8, 2^9): Q's and K's multiply the scores, and
+// V's the weights before these are split in turn.  A row's own power, and not a
+// tile's, so that a key which a query must not see cannot touch its precision.
+//
+// A block owns 64 rows of one (sequence, KV head): the `group` query heads
+// that share the KV head are rows too, so K and V are read once per group.
+// Keys come in tiles of 32: cp.async brings the FP32 values, each thread splits
+// those that it fetched itself (once per block, where the warps would otherwise
+// each split what they read) into FP16 planes in shared memory, and the copies
+// of the next tile run while the warps work on the planes.
+//
+// The tensor cores truncate when they add to an accumulator, so chains are
+// short: two steps of 16 for the leading products, and their sums are added
+// with rounding.
+//
+// Softmax: weights are relative to a maximum that moves only when a score passes
+// it by more than 4 (in log2), so most tiles need no reduction; likewise the
+// power of two that weight x V's power is taken relative to.
+#include <cuda_fp16.h>
+
+#include "attention_packed.cuh"
+
+namespace ppocr {
+
+namespace {
+
+constexpr int kThreads = 128, kRows = 64, kKeys = 32, kPad = 8;
+constexpr float kSlack = 4.f;
+using Piece = PackedPiece<kRows>;
+static_assert(kRows == 2 * kKeys, "Q's rows pass through the same staging as a tile's K and V rows");
+
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same onto zeros: the first step of a chain.
+__device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+__device__ __forceinline__ float power(int e) { return __int_as_float((127 + e) << 23); }   // 2^e, -126 <= e <= 127
+__device__ __forceinline__ int exponent(float x) { return (__float_as_int(x) >> 23) - 127; }   // of x >= 0
+
+// a and b as FP16 pairs: the values rounded, and what is left.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// 64 rows on their way to FP16 planes.  kLanes threads share a row; a thread's
+// pieces of 16 bytes lie at raw[piece x kThreads + thread], for it alone.
+template <int DP>
+struct Rows {
+    static constexpr int kLanes = DP >= 32 ? 8 : 4, kPieces = DP / 4 / kLanes, kPerPass = kThreads / kLanes;
+    static constexpr int kPasses = kRows / kPerPass, kPitch = DP + kPad;
+    static constexpr int kRawBytes = kRows * DP * 4, kPlaneBytes = kRows * kPitch * 2;
+
+    // row(n): row n's values, null for zeros; `any` is readable.
+    template <typename Row>
+    static __device__ __forceinline__ void fetch(float4* raw, Row row, const float* any, int d, bool vec) {
+        const int tid = threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const float* src = row(tid / kLanes + kPerPass * i);
+#pragma unroll
+            for (int j = 0; j < kPieces; ++j) {
+                const int x = (tid % kLanes + kLanes * j) * 4;
+                float4* dst = raw + (i * kPieces + j) * kThreads + tid;
+                if (vec) {
+                    const bool live = src && x < d;
+                    cp_async16(dst, live ? src + x : any, live);
+                } else {
+                    const int n = src ? d - x : 0;
+                    *dst = make_float4(n > 0 ? src[x] : 0.f, n > 1 ? src[x + 1] : 0.f, n > 2 ? src[x + 2] : 0.f,
+                                       n > 3 ? src[x + 3] : 0.f);
+                }
+            }
+        }
+    }
+    // The rows' planes, and done(n, top, e) by one thread for row n, which holds
+    // its values times 2^(8 - e); top is its largest magnitude.
+    template <typename Done>
+    static __device__ __forceinline__ void split(const float4* raw, __half* hi, __half* lo, Done done) {
+        const int tid = threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            float4 x[kPieces];
+            float top = 0.f;
+#pragma unroll
+            for (int j = 0; j < kPieces; ++j) {
+                x[j] = raw[(i * kPieces + j) * kThreads + tid];
+                top = fmaxf(fmaxf(top, fmaxf(fabsf(x[j].x), fabsf(x[j].y))), fmaxf(fabsf(x[j].z), fabsf(x[j].w)));
+            }
+#pragma unroll
+            for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const int e = min(max(exponent(top), -100), 120), n = tid / kLanes + kPerPass * i;
+            const float up = power(8 - e);
+#pragma unroll
+            for (int j = 0; j < kPieces; ++j) {
+                uint2 h, l;
+                split2(x[j].x * up, x[j].y * up, h.x, l.x);
+                split2(x[j].z * up, x[j].w * up, h.y, l.y);
+                const int at = n * kPitch + (tid % kLanes + kLanes * j) * 4;
+                *reinterpret_cast<uint2*>(hi + at) = h;
+                *reinterpret_cast<uint2*>(lo + at) = l;
+            }
+            if (tid % kLanes == 0) done(n, top, e);
+        }
+    }
+};
+
+// What a row of Q or K was divided by.  Rows of 2^60 and more are left to
+// attend_row: the factors' product might overflow where the score does not.
+__device__ __forceinline__ float score_factor(float top, int e) { return top < power(60) ? power(e - 8) : NAN; }
+
+template <int DP>
+__global__ void __launch_bounds__(kThreads, DP > 64 ? 2 : DP > 32 ? 4 : 5)
+    attention_packed_f32_kernel(PackedAttentionParams p, bool vec, bool vec_out) {
+    using R = Rows<DP>;
+    constexpr int P = R::kPitch, NT = kKeys / 8, KS = DP / 16, DT = DP / 8;
+    extern __shared__ uint4 smem16[];
+    float4* raw = reinterpret_cast<float4*>(smem16);
+    __half* qh = reinterpret_cast<__half*>(reinterpret_cast<char*>(smem16) + R::kRawBytes);
+    __half* ql = qh + kRows * P;
+    __half* hi = ql + kRows * P;         // a tile's K rows, then its V rows
+    __half* lo = hi + kRows * P;
+    float* fq = reinterpret_cast<float*>(lo + kRows * P);   // [kRows] factors of Q's rows
+    float* fk = fq + kRows;                                 // [kKeys] of K's, then [kKeys] powers of V's rows
+    float* fv = fk + kKeys;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+    const Piece at(p);
+    const int rows = at.rows, d = p.d;
+    if (rows <= 0) return;
+    const int keys = at.keys_of(rows - 1);
+    const int tiles = (keys + kKeys - 1) / kKeys;
+
+    const float* q = at.queries<float>(p.q);
+    const float* k = at.keys<float>(p.k);
+    const float* v = at.keys<float>(p.v);
+    auto fetch_keys = [&](int j) {
+        R::fetch(raw, [&](int n) {
+            const int key = j * kKeys + n % kKeys;
+            const float* src = n < kKeys ? k + key * p.k.token_stride : v + key * p.v.token_stride;
+            return key < keys ? src : nullptr;
+        }, q, d, vec);
+    };
+    float4* raw_q = reinterpret_cast<float4*>(hi);   // until the first tile's planes
+    R::fetch(raw_q, [&](int n) { return n < rows ? q + at.row_at(p.q, n) : nullptr; }, q, d, vec);
+    if (tiles > 0) fetch_keys(0);
+    cp_async_commit();
+    cp_async_wait<0>();
+    R::split(raw_q, qh, ql, [&](int n, float top, int e) { fq[n] = score_factor(top, e); });
+    __syncthreads();
+
+    const float scale = p.scale * 1.4426950408889634f;
+    const int n0 = warp * 16 + r;                  // this lane's rows: n0 and n0 + 8
+    const int keys0 = at.keys_of(min(n0, rows - 1)), keys1 = at.keys_of(min(n0 + 8, rows - 1));
+    const int sure = __reduce_min_sync(0xffffffffu, (unsigned)min(keys0, keys1));   // keys every row of the warp sees
+    const int most = n0 - r < rows ? (int)__reduce_max_sync(0xffffffffu, (unsigned)max(keys0, keys1)) : 0;
+    const float f0 = fq[n0] * scale, f1 = fq[n0 + 8] * scale;
+    float o[DT][4];
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[i][x] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, b0 = 0.f, b1 = 0.f, l0 = 0.f, l1 = 0.f;   // b: m, 0 while it is -infinity
+    int e0 = -100, e1 = -100;            // o holds sums of weight x V, times 2^(16 - e)
+    float unit0 = power(108), unit1 = power(108);   // 2^(8 - e)
+
+    for (int j = 0; j < tiles; ++j) {
+        cp_async_wait<0>();
+        R::split(raw, hi, lo, [&](int n, float top, int e) { fk[n] = n < kKeys ? score_factor(top, e) : power(e); });
+        if (j + 1 < tiles) fetch_keys(j + 1);
+        cp_async_commit();
+        __syncthreads();
+        if (j * kKeys < most) {
+            float s[NT][4], rest[NT][4];
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                uint32_t ah[4], al[4];
+                const int qa = (warp * 16 + (lane & 15)) * P + i * 16 + (lane >> 4) * 8;
+                ldmatrix4(ah, qh + qa);
+                ldmatrix4(al, ql + qa);
+#pragma unroll
+                for (int n = 0; n < NT; n += 2) {
+                    uint32_t bh[4], bl[4];
+                    const int kb = (n * 8 + (lane & 7) + (lane >> 4) * 8) * P + i * 16 + ((lane >> 3) & 1) * 8;
+                    ldmatrix4(bh, hi + kb);
+                    ldmatrix4(bl, lo + kb);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        float part[4];
+                        if (i == 0) mma_first(rest[n + u], al, bh[2 * u], bh[2 * u + 1]);
+                        else mma(rest[n + u], al, bh[2 * u], bh[2 * u + 1]);
+                        mma(rest[n + u], ah, bl[2 * u], bl[2 * u + 1]);
+                        if (i == 0) {
+                            mma_first(s[n + u], ah, bh[2 * u], bh[2 * u + 1]);
+                        } else {
+                            mma_first(part, ah, bh[2 * u], bh[2 * u + 1]);
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) s[n + u][x] += part[x];
+                        }
+                    }
+                }
+            }
+            // Scale, mask; the maximum, where a score passes it by far.
+            float t0 = -INFINITY, t1 = -INFINITY;
+            const bool whole = (j + 1) * kKeys <= sure;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float2 f = *reinterpret_cast<const float2*>(fk + n * 8 + 2 * c);
+                const int key = j * kKeys + n * 8 + 2 * c;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const float fx = x ? f.y : f.x;
+                    s[n][x] = whole || key + x < keys0 ? (s[n][x] + rest[n][x]) * (f0 * fx) : -INFINITY;
+                    s[n][x + 2] = whole || key + x < keys1 ? (s[n][x + 2] + rest[n][x + 2]) * (f1 * fx) : -INFINITY;
+                    t0 = fmaxf(t0, s[n][x]);
+                    t1 = fmaxf(t1, s[n][x + 2]);
+                }
+            }
+            if (__any_sync(0xffffffffu, t0 > m0 + kSlack || t1 > m1 + kSlack)) {
+                auto raise = [&](float t, float& m, float& b, float& l, int& e, float& unit, int half) {
+                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+                    t = fmaxf(m, fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2)));
+                    if (t > m) {   // the whole row's four lanes
+                        // What the sums hold shrinks with the weights, so their power may fall as far.
+                        const float fall = m - t;   // -infinity for the first keys
+                        const int next = max(e + (int)fmaxf(ceilf(fall), -300.f), -100);
+                        const float back = exp2_hw(fall + (float)(e - next));
+                        l *= exp2_hw(fall);
+#pragma unroll
+                        for (int i = 0; i < DT; ++i) {
+                            o[i][half] *= back;
+                            o[i][half + 1] *= back;
+                        }
+                        e = next;
+                        unit = power(8 - e);
+                        b = m = t;
+                    }
+                };
+                raise(t0, m0, b0, l0, e0, unit0, 0);
+                raise(t1, m1, b1, l1, e1, unit1, 2);
+            }
+            // Weights, times the powers of the V rows.
+            float y0 = 0.f, y1 = 0.f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float2 f = *reinterpret_cast<const float2*>(fv + n * 8 + 2 * c);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    s[n][x] = exp2_hw(s[n][x] - b0);
+                    s[n][x + 2] = exp2_hw(s[n][x + 2] - b1);
+                    l0 += s[n][x];
+                    l1 += s[n][x + 2];
+                    s[n][x] *= x ? f.y : f.x;
+                    s[n][x + 2] *= x ? f.y : f.x;
+                    y0 = fmaxf(y0, s[n][x]);
+                    y1 = fmaxf(y1, s[n][x + 2]);
+                }
+            }
+            if (__any_sync(0xffffffffu, y0 * unit0 > 32768.f || y1 * unit1 > 32768.f)) {
+                auto raise = [&](float y, int& e, float& unit, int half) {
+                    y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
+                    y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
+                    const int next = min(max(e, exponent(y) + 1), 126), by = max(e - next, -126);   // sums of 2^-126 are none
+                    const float back = power(by);
+#pragma unroll
+                    for (int i = 0; i < DT; ++i) {
+                        o[i][half] *= back;
+                        o[i][half + 1] *= back;
+                    }
+                    e = next;
+                    unit = power(8 - e);
+                };
+                raise(y0, e0, unit0, 0);
+                raise(y1, e1, unit1, 2);
+            }
+            uint32_t wh[NT / 2][4], wl[NT / 2][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                split2(s[n][0] * unit0, s[n][1] * unit0, wh[n / 2][n % 2 * 2], wl[n / 2][n % 2 * 2]);
+                split2(s[n][2] * unit1, s[n][3] * unit1, wh[n / 2][n % 2 * 2 + 1], wl[n / 2][n % 2 * 2 + 1]);
+            }
+#pragma unroll
+            for (int i = 0; i < DT; i += 2) {
+                uint32_t bh[NT / 2][4], bl[NT / 2][4];
+#pragma unroll
+                for (int n = 0; n < NT / 2; ++n) {
+                    const int vb = (kKeys + n * 16 + (lane & 15)) * P + i * 8 + (lane >> 4) * 8;
+                    ldmatrix4_trans(bh[n], hi + vb);
+                    ldmatrix4_trans(bl[n], lo + vb);
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float sum[4];   // the small products first
+                    mma_first(sum, wl[0], bh[0][2 * u], bh[0][2 * u + 1]);
+                    mma(sum, wh[0], bl[0][2 * u], bl[0][2 * u + 1]);
+#pragma unroll
+                    for (int n = 1; n < NT / 2; ++n) {
+                        mma(sum, wl[n], bh[n][2 * u], bh[n][2 * u + 1]);
+                        mma(sum, wh[n], bl[n][2 * u], bl[n][2 * u + 1]);
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT / 2; ++n) mma(sum, wh[n], bh[n][2 * u], bh[n][2 * u + 1]);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) o[i + u][x] += sum[x];
+                }
+            }
+        }
+        __syncthreads();
+    }
+
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
+    const float u0 = power(e0 - 16), u1 = power(e1 - 16);
+    float* out = at.queries<float>(p.out);
+    bool bad[2] = {false, false};
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int n = n0 + 8 * half;
+        if (n >= rows) continue;
+        float* dst = out + at.row_at(p.out, n);
+        const float inv = half ? i1 : i0, unit = half ? u1 : u0;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+            const int x = i * 8 + 2 * c;
+            const float a = o[i][2 * half] * inv * unit, b = o[i][2 * half + 1] * inv * unit;
+            bad[half] |= (x < d && !isfinite(a)) || (x + 1 < d && !isfinite(b));
+            if (vec_out && x + 1 < d) {
+                *reinterpret_cast<float2*>(dst + x) = make_float2(a, b);
+            } else {
+                if (x < d) dst[x] = a;
+                if (x + 1 < d) dst[x + 1] = b;
+            }
+        }
+    }
+    // Rows with a non-finite value again, by their definition, after the
+    // warp's own stores above.  A row is shared by four lanes.
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const unsigned again = __ballot_sync(0xffffffffu, bad[half]);
+        for (int rr = 0; again && rr < 8; ++rr) {
+            if (!(again >> (4 * rr) & 0xfu)) continue;
+            const int n = warp * 16 + rr + 8 * half;
+            __syncwarp();
+            attend_row<float>(q + at.row_at(p.q, n), k, p.k.token_stride, v, p.v.token_stride, d, at.keys_of(n), scale,
+                              out + at.row_at(p.out, n));
+        }
+    }
+}
+
+template <int DP>
+cudaError_t launch_dp(const PackedAttentionParams& p, cudaStream_t stream) {
+    const bool vec = rows16(p.q, 4) && rows16(p.k, 4) && rows16(p.v, 4) && p.d % 4 == 0;
+    constexpr int smem = Rows<DP>::kRawBytes + 4 * Rows<DP>::kPlaneBytes + (kRows + 2 * kKeys) * 4;
+    cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(attention_packed_f32_kernel<DP>), smem);
+    if (e != cudaSuccess) return e;
+    attention_packed_f32_kernel<DP><<<(unsigned)Piece::blocks(p), kThreads, smem, stream>>>(p, vec, pairs_aligned(p.out, 4));
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_attention_packed_f32(const PackedAttentionParams& p, cudaStream_t stream) {
+    if (p.d <= 16) return launch_dp<16>(p, stream);
+    if (p.d <= 32) return launch_dp<32>(p, stream);
+    if (p.d <= 64) return launch_dp<64>(p, stream);
+    return launch_dp<128>(p, stream);
+}
+
+}  // namespace ppocr

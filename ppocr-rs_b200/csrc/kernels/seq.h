@@ -45,6 +45,7 @@ struct PackedAttentionParams {
 };
 constexpr int kPackedMaxD = 128;
 cudaError_t launch_attention_packed(const PackedAttentionParams& p, cudaStream_t stream);
+cudaError_t launch_attention_packed_f32(const PackedAttentionParams& p, cudaStream_t stream);   // DT_F32, not empty
 
 // Its tcgen05 kernel (attention_tc.cu): BF16, 16-byte aligned rows, d a multiple
 // of 8 and at most 128 query heads to a KV head.
