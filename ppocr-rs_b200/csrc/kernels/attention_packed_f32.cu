@@ -20,6 +20,12 @@
 // short: two steps of 16 for the leading products, and their sums are added
 // with rounding.
 //
+// Bound: the tensor cores (three products) together with splitting, 1 us of
+// every 4 where it stood between two barriers; with eight warps one half of
+// them splits the next tile while the other half multiplies (95 -> 89 us).
+// Chunks of 3 requests, 16 heads of 64, 4 KV heads: 78 us (TF32 pieces split by
+// each warp: 165).  64 lines of 4 to 200 tokens, 8 heads of 15: 30 us, latency.
+//
 // Softmax: weights are relative to a maximum that moves only when a score passes
 // it by more than 4 (in log2), so most tiles need no reduction; likewise the
 // power of two that weight x V's power is taken relative to.
@@ -31,10 +37,8 @@ namespace ppocr {
 
 namespace {
 
-constexpr int kThreads = 128, kRows = 64, kKeys = 32, kPad = 8;
+constexpr int kKeys = 32, kPad = 8;
 constexpr float kSlack = 4.f;
-using Piece = PackedPiece<kRows>;
-static_assert(kRows == 2 * kKeys, "Q's rows pass through the same staging as a tile's K and V rows");
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -62,13 +66,16 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// 64 rows on their way to FP16 planes.  kLanes threads share a row; a thread's
-// pieces of 16 bytes lie at raw[piece x kThreads + thread], for it alone.
-template <int DP>
+// ROWS rows on their way to FP16 planes by a block of WARPS warps.  kLanes threads
+// share a row; a thread's pieces of 16 bytes lie at raw[piece x kThreads + thread],
+// for it alone.
+template <int DP, int WARPS, int ROWS>
 struct Rows {
+    static constexpr int kThreads = 32 * WARPS, kPitch = DP + kPad;
     static constexpr int kLanes = DP >= 32 ? 8 : 4, kPieces = DP / 4 / kLanes, kPerPass = kThreads / kLanes;
-    static constexpr int kPasses = kRows / kPerPass, kPitch = DP + kPad;
-    static constexpr int kRawBytes = kRows * DP * 4, kPlaneBytes = kRows * kPitch * 2;
+    static constexpr int kPasses = ROWS / kPerPass;
+    static constexpr int kRawBytes = ROWS * DP * 4, kPlaneBytes = ROWS * kPitch * 2;
+    static_assert(kPasses * kPerPass == ROWS, "whole passes");
 
     // row(n): row n's values, null for zeros; `any` is readable.
     template <typename Row>
@@ -128,30 +135,41 @@ struct Rows {
 // attend_row: the factors' product might overflow where the score does not.
 __device__ __forceinline__ float score_factor(float top, int e) { return top < power(60) ? power(e - 8) : NAN; }
 
-template <int DP>
-__global__ void __launch_bounds__(kThreads, DP > 64 ? 2 : DP > 32 ? 4 : 5)
+// What a block of WARPS warps, 16 rows each, keeps in shared memory.  With two
+// buffers of planes the next tile is split while this one is worked on.
+template <int DP, int WARPS>
+struct Plan {
+    static constexpr int kRows = 16 * WARPS, kBuffers = DP > 64 && WARPS == 4 ? 1 : 2;
+    using Q = Rows<DP, WARPS, kRows>;
+    using KV = Rows<DP, WARPS, 2 * kKeys>;   // a tile's K rows, then its V rows
+    static constexpr int kPlanes = 2 * KV::kPlaneBytes, kFactors = 2 * kKeys * 4;
+    static constexpr int kBytes = KV::kRawBytes + 2 * Q::kPlaneBytes + kBuffers * (kPlanes + kFactors) + kRows * 4;
+    static_assert(Q::kRawBytes <= kBuffers * kPlanes, "Q is staged where the planes will be");
+};
+
+template <int DP, int WARPS, int BLOCKS>
+__global__ void __launch_bounds__(32 * WARPS, BLOCKS)
     attention_packed_f32_kernel(PackedAttentionParams p, bool vec, bool vec_out) {
-    using R = Rows<DP>;
-    constexpr int P = R::kPitch, NT = kKeys / 8, KS = DP / 16, DT = DP / 8;
+    using L = Plan<DP, WARPS>;
+    using R = typename L::KV;
+    constexpr int P = R::kPitch, NT = kKeys / 8, KS = DP / 16, DT = DP / 8, kRows = L::kRows;
     extern __shared__ uint4 smem16[];
     float4* raw = reinterpret_cast<float4*>(smem16);
     __half* qh = reinterpret_cast<__half*>(reinterpret_cast<char*>(smem16) + R::kRawBytes);
     __half* ql = qh + kRows * P;
-    __half* hi = ql + kRows * P;         // a tile's K rows, then its V rows
-    __half* lo = hi + kRows * P;
-    float* fq = reinterpret_cast<float*>(lo + kRows * P);   // [kRows] factors of Q's rows
-    float* fk = fq + kRows;                                 // [kKeys] of K's, then [kKeys] powers of V's rows
-    float* fv = fk + kKeys;
+    __half* planes = ql + kRows * P;     // per buffer the first pieces, then the second
+    float* fq = reinterpret_cast<float*>(reinterpret_cast<char*>(planes) + L::kBuffers * L::kPlanes);   // factors of Q's rows
+    float* factors = fq + kRows;         // per buffer those of K's rows, then the powers of V's
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-    const Piece at(p);
+    const PackedPiece<kRows> at(p);
     const int rows = at.rows, d = p.d;
     if (rows <= 0) return;
     const int keys = at.keys_of(rows - 1);
     const int tiles = (keys + kKeys - 1) / kKeys;
 
-    const float* q = at.queries<float>(p.q);
-    const float* k = at.keys<float>(p.k);
-    const float* v = at.keys<float>(p.v);
+    const float* q = at.template queries<float>(p.q);
+    const float* k = at.template keys<float>(p.k);
+    const float* v = at.template keys<float>(p.v);
     auto fetch_keys = [&](int j) {
         R::fetch(raw, [&](int n) {
             const int key = j * kKeys + n % kKeys;
@@ -159,13 +177,24 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 2 : DP > 32 ? 4 : 5)
             return key < keys ? src : nullptr;
         }, q, d, vec);
     };
-    float4* raw_q = reinterpret_cast<float4*>(hi);   // until the first tile's planes
-    R::fetch(raw_q, [&](int n) { return n < rows ? q + at.row_at(p.q, n) : nullptr; }, q, d, vec);
+    float4* raw_q = reinterpret_cast<float4*>(planes);   // until the first tile's planes
+    L::Q::fetch(raw_q, [&](int n) { return n < rows ? q + at.row_at(p.q, n) : nullptr; }, q, d, vec);
     if (tiles > 0) fetch_keys(0);
     cp_async_commit();
     cp_async_wait<0>();
-    R::split(raw_q, qh, ql, [&](int n, float top, int e) { fq[n] = score_factor(top, e); });
+    L::Q::split(raw_q, qh, ql, [&](int n, float top, int e) { fq[n] = score_factor(top, e); });
     __syncthreads();
+    // Tile j, whose copies are the last that were started, into its planes; starts the next one's.
+    auto split_keys = [&](int j) {
+        cp_async_wait<0>();
+        const int at_buffer = j % L::kBuffers;
+        __half* hi = planes + at_buffer * (L::kPlanes / 2);
+        float* f = factors + at_buffer * (2 * kKeys);
+        R::split(raw, hi, hi + 2 * kKeys * P,
+                 [&](int n, float top, int e) { f[n] = n < kKeys ? score_factor(top, e) : power(e); });
+        if (j + 1 < tiles) fetch_keys(j + 1);
+        cp_async_commit();
+    };
 
     const float scale = p.scale * 1.4426950408889634f;
     const int n0 = warp * 16 + r;                  // this lane's rows: n0 and n0 + 8
@@ -182,12 +211,19 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 2 : DP > 32 ? 4 : 5)
     int e0 = -100, e1 = -100;            // o holds sums of weight x V, times 2^(16 - e)
     float unit0 = power(108), unit1 = power(108);   // 2^(8 - e)
 
-    for (int j = 0; j < tiles; ++j) {
-        cp_async_wait<0>();
-        R::split(raw, hi, lo, [&](int n, float top, int e) { fk[n] = n < kKeys ? score_factor(top, e) : power(e); });
-        if (j + 1 < tiles) fetch_keys(j + 1);
-        cp_async_commit();
+    if (tiles > 0) {
+        split_keys(0);
         __syncthreads();
+    }
+    for (int j = 0; j < tiles; ++j) {
+        const __half* hi = planes + j % L::kBuffers * (L::kPlanes / 2);
+        const __half* lo = hi + 2 * kKeys * P;
+        const float* fk = factors + j % L::kBuffers * (2 * kKeys);
+        const float* fv = fk + kKeys;
+        // With eight warps one half splits the next tile before its work on this
+        // one and the other after it, so that both kinds of work are at hand.
+        const bool late = WARPS == 8 && warp >= 4;
+        if (L::kBuffers > 1 && !late && j + 1 < tiles) split_keys(j + 1);
         if (j * kKeys < most) {
             float s[NT][4], rest[NT][4];
 #pragma unroll
@@ -238,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 2 : DP > 32 ? 4 : 5)
                 auto raise = [&](float t, float& m, float& b, float& l, int& e, float& unit, int half) {
                     t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
                     t = fmaxf(m, fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2)));
-                    if (t > m) {   // the whole row's four lanes
+                    if (t > m + kSlack) {   // the whole row's four lanes; a row's steps depend on its own scores alone
                         // What the sums hold shrinks with the weights, so their power may fall as far.
                         const float fall = m - t;   // -infinity for the first keys
                         const int next = max(e + (int)fmaxf(ceilf(fall), -300.f), -100);
@@ -278,15 +314,17 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 2 : DP > 32 ? 4 : 5)
                 auto raise = [&](float y, int& e, float& unit, int half) {
                     y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
                     y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
-                    const int next = min(max(e, exponent(y) + 1), 126), by = max(e - next, -126);   // sums of 2^-126 are none
-                    const float back = power(by);
+                    if (y * unit > 32768.f) {
+                        const int next = min(max(e, exponent(y) + 1), 126);
+                        const float back = power(max(e - next, -126));   // what 2^-126 leaves of a sum counts for nothing
 #pragma unroll
-                    for (int i = 0; i < DT; ++i) {
-                        o[i][half] *= back;
-                        o[i][half + 1] *= back;
+                        for (int i = 0; i < DT; ++i) {
+                            o[i][half] *= back;
+                            o[i][half + 1] *= back;
+                        }
+                        e = next;
+                        unit = power(8 - e);
                     }
-                    e = next;
-                    unit = power(8 - e);
                 };
                 raise(y0, e0, unit0, 0);
                 raise(y1, e1, unit1, 2);
@@ -323,7 +361,12 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 2 : DP > 32 ? 4 : 5)
                 }
             }
         }
+        if (L::kBuffers > 1 && late && j + 1 < tiles) split_keys(j + 1);
         __syncthreads();
+        if (L::kBuffers == 1 && j + 1 < tiles) {
+            split_keys(j + 1);
+            __syncthreads();
+        }
     }
 
     l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
@@ -332,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 2 : DP > 32 ? 4 : 5)
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
     const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
     const float u0 = power(e0 - 16), u1 = power(e1 - 16);
-    float* out = at.queries<float>(p.out);
+    float* out = at.template queries<float>(p.out);
     bool bad[2] = {false, false};
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -368,14 +411,37 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 2 : DP > 32 ? 4 : 5)
     }
 }
 
+template <int DP, int WARPS, int BLOCKS>
+cudaError_t launch(const PackedAttentionParams& p, cudaStream_t stream) {
+    const bool vec = rows16(p.q, 4) && rows16(p.k, 4) && rows16(p.v, 4) && p.d % 4 == 0;
+    using L = Plan<DP, WARPS>;
+    const auto kernel = attention_packed_f32_kernel<DP, WARPS, BLOCKS>;
+    cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kBytes);
+    if (e != cudaSuccess) return e;
+    kernel<<<(unsigned)PackedPiece<L::kRows>::blocks(p), 32 * WARPS, L::kBytes, stream>>>(p, vec, pairs_aligned(p.out, 4));
+    return cudaGetLastError();
+}
+
+// Blocks of eight warps (128 rows, K and V split half as often) where sequences
+// fill them.  Measured on 8,192 tokens in causal sequences of equal length, four
+// / eight warps in us (rows per sequence: length x heads per KV head):
+//   8 heads of 15          length 64: 20 / 28, 96: 23 / 27, 128: 25 / 25, 1,024: 97 / 85
+//   16 of 32, 4 KV heads   length 64: 36 / 38, 96: 42 / 42, 128: 48 / 46, 1,024: 190 / 164
+//   8 of 64                length 64: 40 / 47, 96: 52 / 45, 128: 49 / 40, 1,024: 184 / 161
+//   16 of 64, 4 KV heads   length 32: 50 / 45, 64: 62 / 50
+//   32 of 128, 8 KV heads  length 32: 180 / 175, 64: 230 / 193, 1,024: 1,061 / 836
+// For d = 64, whose registers two blocks would share, a block has an SM to
+// itself where there are no more blocks than SMs (138 blocks: 78 us, with
+// two 89; 1,024 blocks of 128 keys: 85 us, with two 63).
 template <int DP>
 cudaError_t launch_dp(const PackedAttentionParams& p, cudaStream_t stream) {
-    const bool vec = rows16(p.q, 4) && rows16(p.k, 4) && rows16(p.v, 4) && p.d % 4 == 0;
-    constexpr int smem = Rows<DP>::kRawBytes + 4 * Rows<DP>::kPlaneBytes + (kRows + 2 * kKeys) * 4;
-    cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(attention_packed_f32_kernel<DP>), smem);
-    if (e != cudaSuccess) return e;
-    attention_packed_f32_kernel<DP><<<(unsigned)Piece::blocks(p), kThreads, smem, stream>>>(p, vec, pairs_aligned(p.out, 4));
-    return cudaGetLastError();
+    const long long rows = (long long)p.total_q * (p.heads / p.kv_heads);
+    const bool full = DP > 32 ? rows >= 96ll * p.sequences : rows >= 128ll * p.sequences && p.total_k >= 128ll * p.sequences;
+    if (!full) return launch<DP, 4, (DP > 64 ? 2 : DP > 32 ? 3 : 5)>(p, stream);
+    if constexpr (DP == 64) {
+        if (rows * p.kv_heads <= 128ll * 148) return launch<DP, 8, 1>(p, stream);
+    }
+    return launch<DP, 8, (DP > 64 ? 1 : 2)>(p, stream);
 }
 
 }  // namespace

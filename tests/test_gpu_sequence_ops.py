@@ -148,6 +148,51 @@ def test_packed_long_groups(gpu, heads, kv, causal):
     run_packed(gpu, [257, 1, 300], [400, 500, 300], heads, kv, 64, "bf16", causal, seed=heads)
 
 
+@pytest.mark.parametrize("d", [1, 15, 16, 31, 32, 33, 64, 72, 127, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_packed_long_fp32(gpu, d, causal):
+    run_packed(gpu, [300, 555, 128, 0, 257], [300, 600, 160, 40, 250], 4, 2, d, "f32", causal, seed=d)
+
+
+@pytest.mark.parametrize("d", [24, 64, 128])
+def test_packed_many_long_fp32(gpu, d):   # more blocks than SMs
+    run_packed(gpu, [1000, 1201, 900], [1000, 1201, 900], 8, 2, d, "f32", True, seed=d)
+
+
+@pytest.mark.parametrize("n", [40, 300])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("powers", [(0, 0, 60), (0, 10, 60), (64, 0, 0), (-64, 0, 30)])
+def test_packed_fp32_rows_of_different_powers(gpu, n, causal, powers):
+    """Rows of V up to 2^+-60 apart, keys of 2^-10 to 1 of the others, and q and k far from 1 (2^64 among them,
+    whose rows are computed from their definition)."""
+    shift, below, apart = powers
+    g = rng(n + apart)
+    q, k, v = (torch.randn(n, h, 48, device="cuda", generator=g) for h in (4, 2, 2))
+    q, k = q * 2.0 ** -shift, k * 2.0 ** shift
+    k *= torch.exp2(-torch.randint(0, below + 1, (n, 2, 1), device="cuda", generator=g).float())
+    v *= torch.exp2(torch.randint(-apart, apart + 1, (n, 2, 1), device="cuda", generator=g).float())
+    out = torch.empty_like(q)
+    gpu.attention_packed(q, k, v, offsets([n]), offsets([n]), out, causal=causal, stream=torch.cuda.current_stream())
+    gpu.synchronize(torch.cuda.current_stream())
+    ref, tol = packed_reference(q, k, v, [n], [n], causal, 48 ** -0.5, "f32")
+    check(out, ref, tol, f"{n} {powers}")
+
+
+@pytest.mark.parametrize("n,heads", [(50, 2), (200, 2), (200, 8)])
+def test_packed_fp32_later_keys_change_no_bit(gpu, n, heads):
+    g = rng(n)
+    q, k, v = (torch.randn(n, h, 64, device="cuda", generator=g) for h in (heads, 2, 2))
+    outs = []
+    for keep in (n, n - 21):
+        k[keep:] *= 1e15
+        v[keep:] *= 1e30
+        outs.append(torch.empty_like(q))
+        gpu.attention_packed(q, k, v, offsets([n]), offsets([n]), outs[-1], causal=True,
+                             stream=torch.cuda.current_stream())
+    gpu.synchronize(torch.cuda.current_stream())
+    assert torch.equal(outs[0][:n - 21], outs[1][:n - 21])
+
+
 @pytest.mark.parametrize("nq,nk", [([1], [256]), ([128, 256], [512, 256]), ([127, 129, 0, 255], [383, 385, 700, 257]),
                                    ([640, 10, 700], [0, 3, 900]), ([2000], [2000]), ([1, 3, 5], [5000, 300, 1025]),
                                    ([1100, 3, 900], [1100, 1400, 900]), ([333] * 40, [333] * 40)])
