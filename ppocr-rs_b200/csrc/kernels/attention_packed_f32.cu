@@ -430,16 +430,21 @@ cudaError_t launch(const PackedAttentionParams& p, cudaStream_t stream) {
 //   8 of 64                length 64: 40 / 47, 96: 52 / 45, 128: 49 / 40, 1,024: 184 / 161
 //   16 of 64, 4 KV heads   length 32: 50 / 45, 64: 62 / 50
 //   32 of 128, 8 KV heads  length 32: 180 / 175, 64: 230 / 193, 1,024: 1,061 / 836
-// For d = 64, whose registers two blocks would share, a block has an SM to
-// itself where there are no more blocks than SMs (138 blocks: 78 us, with
-// two 89; 1,024 blocks of 128 keys: 85 us, with two 63).
+// For d = 64, where two blocks on an SM have to share its registers, a block has
+// an SM to itself up to 1.5 x 148 blocks: each is faster, and the last ones, the
+// shortest of causal sequences, start where others end.  16 heads, 4 KV heads,
+// alone / two per SM in us:
+//   1,024 tokens (128 blocks)  length 128: 15 / 18, 512: 38 / 39
+//   1,480 tokens (185)         length 92: 20 / 18, 185: 26 / 27, 370: 35 / 44, 740: 51 / 64
+//   2,220 tokens (277)         length 138: 31 / 25, 277: 42 / 36, 555: 64 / 64, 1,110: 78 / 116
+//   2,960 tokens (370)         length 185: 42 / 37, 370: 59 / 54, 740: 91 / 77, 1,480: 142 / 146
 template <int DP>
 cudaError_t launch_dp(const PackedAttentionParams& p, cudaStream_t stream) {
     const long long rows = (long long)p.total_q * (p.heads / p.kv_heads);
     const bool full = DP > 32 ? rows >= 96ll * p.sequences : rows >= 128ll * p.sequences && p.total_k >= 128ll * p.sequences;
     if (!full) return launch<DP, 4, (DP > 64 ? 2 : DP > 32 ? 3 : 5)>(p, stream);
     if constexpr (DP == 64) {
-        if (rows * p.kv_heads <= 128ll * 148) return launch<DP, 8, 1>(p, stream);
+        if (rows * p.kv_heads <= 128ll * 222) return launch<DP, 8, 1>(p, stream);
     }
     return launch<DP, 8, (DP > 64 ? 1 : 2)>(p, stream);
 }

@@ -7,6 +7,11 @@
 // and stays in registers; with a history a block owns one chunk of one row and
 // counts the chunk's ids in shared memory first (integer counts, so the order
 // of the atomics does not matter).
+//
+// Measured: 10,240 x 6,906 in FP32, bias and one mask: 113 us (5.0 TB/s; one row in
+// flight per thread: 142); 64 x 128,000 in BF16 with histories of up to 4,000 ids:
+// 20 us (1.7 TB/s; scalar reads of bias and counts: 26), where clearing, filling
+// and reading the counts stand before and between the loads.
 #include "seq_common.cuh"
 
 namespace ppocr {
