@@ -76,8 +76,8 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 6)
         const int n = min(BN, keys - j * BN);
         const T* kt = k + (long long)j * BN * p.k.token_stride;
         const T* vt = v + (long long)j * BN * p.v.token_stride;
-        load_tile<DP>(sk + (j & 1) * BN * P, kt, [&](int i) { return i * p.k.token_stride; }, BN, n, d, vec);
-        load_tile<DP>(sv + (j & 1) * BN * P, vt, [&](int i) { return i * p.v.token_stride; }, BN, n, d, vec);
+        load_tile<DP>(sk + (j & 1) * BN * P, kt, [&](int i) { return (long long)i * (int)p.k.token_stride; }, BN, n, d, vec);
+        load_tile<DP>(sv + (j & 1) * BN * P, vt, [&](int i) { return (long long)i * (int)p.v.token_stride; }, BN, n, d, vec);
     };
     if (tiles > 0) load_keys(0);
     cp_async_commit();
@@ -129,27 +129,34 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 6)
                 mma_bf16_16816(s[n + 1], qf[i], b[2], b[3]);
             }
         }
-        // Scale, mask, running maximum.
+        // Mask, running maximum (of the products; the scale, which is positive,
+        // comes with the exponent's subtraction).
         float t0 = -INFINITY, t1 = -INFINITY;
-        const bool whole = (j + 1) * BN <= sure;
+        if ((j + 1) * BN > sure) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                if (n >= (seen + 1) / 2 * 2) break;   // they come in pairs
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int key = j * BN + n * 8 + 2 * c + x;
+                    if (key >= keys0) s[n][x] = -INFINITY;
+                    if (key >= keys1) s[n][x + 2] = -INFINITY;
+                }
+            }
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            if (n >= (seen + 1) / 2 * 2) break;   // they come in pairs
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int key = j * BN + n * 8 + 2 * c + x;
-                s[n][x] = whole || key < keys0 ? s[n][x] * scale : -INFINITY;
-                s[n][x + 2] = whole || key < keys1 ? s[n][x + 2] * scale : -INFINITY;
-                t0 = fmaxf(t0, s[n][x]);
-                t1 = fmaxf(t1, s[n][x + 2]);
-            }
+            if (n >= (seen + 1) / 2 * 2) break;
+            t0 = fmaxf(t0, fmaxf(s[n][0], s[n][1]));
+            t1 = fmaxf(t1, fmaxf(s[n][2], s[n][3]));
         }
         t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1));
         t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
         t0 = fmaxf(m0, fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2)));
         t1 = fmaxf(m1, fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2)));
-        const float b0 = t0 == -INFINITY ? 0.f : t0, b1 = t1 == -INFINITY ? 0.f : t1;
-        const float g0 = exp2_hw(m0 - b0), g1 = exp2_hw(m1 - b1);   // 0 while the maximum is -infinity
+        const float b0 = t0 == -INFINITY ? 0.f : __fmul_rn(t0, scale), b1 = t1 == -INFINITY ? 0.f : __fmul_rn(t1, scale);
+        // 0 while the maximum is -infinity; the products as they were rounded for the weights so far.
+        const float g0 = exp2_hw(__fmul_rn(m0, scale) - b0), g1 = exp2_hw(__fmul_rn(m1, scale) - b1);
         m0 = t0;
         m1 = t1;
         l0 *= g0;
@@ -162,8 +169,8 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 6)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             if (n >= (seen + 1) / 2 * 2) break;
-            s[n][0] = exp2_hw(s[n][0] - b0); s[n][1] = exp2_hw(s[n][1] - b0);
-            s[n][2] = exp2_hw(s[n][2] - b1); s[n][3] = exp2_hw(s[n][3] - b1);
+            s[n][0] = exp2_hw(fmaf(s[n][0], scale, -b0)); s[n][1] = exp2_hw(fmaf(s[n][1], scale, -b0));
+            s[n][2] = exp2_hw(fmaf(s[n][2], scale, -b1)); s[n][3] = exp2_hw(fmaf(s[n][3], scale, -b1));
             l0 += s[n][0] + s[n][1];
             l1 += s[n][2] + s[n][3];
         }
@@ -192,7 +199,8 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 6)
     l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
+    // A maximum whose scaled value overflows leaves sums of 0 or NaN: no number, so the row is computed again.
+    const float i0 = m0 == -INFINITY ? 0.f : 1.f / l0, i1 = m1 == -INFINITY ? 0.f : 1.f / l1;
     T* out = at.queries<T>(p.out);
     bool bad[2] = {false, false};
 #pragma unroll
@@ -200,12 +208,13 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 6)
         const int n = n0 + 8 * half;
         if (n >= rows) continue;
         T* dst = out + at.row_at(p.out, n);
+        float odd = 0.f;   // stays 0, or becomes NaN
         const float inv = half ? i1 : i0;
 #pragma unroll
         for (int i = 0; i < DT; ++i) {
             const int x = i * 8 + 2 * c;
             const float a = o[i][2 * half] * inv, b = o[i][2 * half + 1] * inv;
-            bad[half] |= (x < d && !isfinite(a)) || (x + 1 < d && !isfinite(b));
+            odd = fmaf(a, 0.f, fmaf(b, 0.f, odd));   // columns past d hold zeros
             if (vec_out && x + 1 < d) {
                 *reinterpret_cast<__nv_bfloat162*>(dst + x) = __floats2bfloat162_rn(a, b);
             } else {
@@ -213,6 +222,7 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 6)
                 if (x + 1 < d) dst[x + 1] = from_f<T>(b);
             }
         }
+        bad[half] = odd != 0.f;
     }
     // Rows with a non-finite value again, by their definition, after the
     // warp's own stores above.  A row is shared by four lanes.

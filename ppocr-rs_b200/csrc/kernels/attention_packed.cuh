@@ -68,11 +68,13 @@ struct PackedPiece {
         const long long row0 = (id - first_id(seq)) * ROWS, all = (long long)qs.len * group;
         rows = row0 < 0 ? 0 : (int)max(min((long long)ROWS, all - row0), 0ll);
         shift = ks.len - qs.len;
-        token0 = (int)(row0 / group);
-        part0 = (int)(row0 % group);
+        // Divisions of 64 bits cost as much as a tile of keys.
+        token0 = (int)(group == 1 ? row0 : row0 >> 32 ? row0 / group : (unsigned)row0 / (unsigned)group);
+        part0 = (int)(row0 - (long long)token0 * group);
     }
+    __device__ __forceinline__ int token_of(int n) const { return group == 1 ? n : (part0 + n) / group; }
     __device__ __forceinline__ int keys_of(int n) const {
-        return causal ? min(max(token0 + (part0 + n) / group + shift + 1, 0), ks.len) : ks.len;
+        return causal ? min(max(token0 + token_of(n) + shift + 1, 0), ks.len) : ks.len;
     }
     template <typename T>
     __device__ __forceinline__ T* queries(const SeqTensor& t) const {
@@ -83,8 +85,8 @@ struct PackedPiece {
         return static_cast<const T*>(t.ptr) + (long long)ks.begin * t.token_stride + kv * t.head_stride;
     }
     __device__ __forceinline__ long long row_at(const SeqTensor& t, int n) const {
-        const int x = part0 + n;
-        return (long long)(x / group) * t.token_stride + (x % group) * t.head_stride;
+        const int token = token_of(n);   // strides are at most 2^30: products of 32 bits
+        return (long long)token * (int)t.token_stride + (long long)(part0 + n - token * group) * (int)t.head_stride;
     }
     // Blocks of a launch: sequence i owns the ids from floor(offset_i group / ROWS) + i, at least its number of pieces.
     static long long blocks(const PackedAttentionParams& p) {
@@ -95,6 +97,10 @@ struct PackedPiece {
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool live) {
     const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(void* dst, const void* src, bool live) {
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(src), "r"(live ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }

@@ -93,8 +93,8 @@ struct Rows {
                     cp_async16(dst, live ? src + x : any, live);
                 } else {
                     const int n = src ? d - x : 0;
-                    *dst = make_float4(n > 0 ? src[x] : 0.f, n > 1 ? src[x + 1] : 0.f, n > 2 ? src[x + 2] : 0.f,
-                                       n > 3 ? src[x + 3] : 0.f);
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) cp_async4(&dst->x + u, n > u ? src + x + u : any, n > u);
                 }
             }
         }
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS)
     auto fetch_keys = [&](int j) {
         R::fetch(raw, [&](int n) {
             const int key = j * kKeys + n % kKeys;
-            const float* src = n < kKeys ? k + key * p.k.token_stride : v + key * p.v.token_stride;
+            const float* src = n < kKeys ? k + (long long)key * (int)p.k.token_stride : v + (long long)key * (int)p.v.token_stride;
             return key < keys ? src : nullptr;
         }, q, d, vec);
     };
@@ -256,19 +256,30 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS)
             }
             // Scale, mask; the maximum, where a score passes it by far.
             float t0 = -INFINITY, t1 = -INFINITY;
-            const bool whole = (j + 1) * kKeys <= sure;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const float2 f = *reinterpret_cast<const float2*>(fk + n * 8 + 2 * c);
-                const int key = j * kKeys + n * 8 + 2 * c;
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     const float fx = x ? f.y : f.x;
-                    s[n][x] = whole || key + x < keys0 ? (s[n][x] + rest[n][x]) * (f0 * fx) : -INFINITY;
-                    s[n][x + 2] = whole || key + x < keys1 ? (s[n][x + 2] + rest[n][x + 2]) * (f1 * fx) : -INFINITY;
-                    t0 = fmaxf(t0, s[n][x]);
-                    t1 = fmaxf(t1, s[n][x + 2]);
+                    s[n][x] = (s[n][x] + rest[n][x]) * (f0 * fx);
+                    s[n][x + 2] = (s[n][x + 2] + rest[n][x + 2]) * (f1 * fx);
                 }
+            }
+            if ((j + 1) * kKeys > sure) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int key = j * kKeys + n * 8 + 2 * c + x;
+                        if (key >= keys0) s[n][x] = -INFINITY;
+                        if (key >= keys1) s[n][x + 2] = -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                t0 = fmaxf(t0, fmaxf(s[n][0], s[n][1]));
+                t1 = fmaxf(t1, fmaxf(s[n][2], s[n][3]));
             }
             if (__any_sync(0xffffffffu, t0 > m0 + kSlack || t1 > m1 + kSlack)) {
                 auto raise = [&](float t, float& m, float& b, float& l, int& e, float& unit, int half) {
@@ -382,12 +393,13 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS)
         const int n = n0 + 8 * half;
         if (n >= rows) continue;
         float* dst = out + at.row_at(p.out, n);
+        float odd = 0.f;   // stays 0, or becomes NaN
         const float inv = half ? i1 : i0, unit = half ? u1 : u0;
 #pragma unroll
         for (int i = 0; i < DT; ++i) {
             const int x = i * 8 + 2 * c;
             const float a = o[i][2 * half] * inv * unit, b = o[i][2 * half + 1] * inv * unit;
-            bad[half] |= (x < d && !isfinite(a)) || (x + 1 < d && !isfinite(b));
+            odd = fmaf(a, 0.f, fmaf(b, 0.f, odd));   // columns past d hold zeros
             if (vec_out && x + 1 < d) {
                 *reinterpret_cast<float2*>(dst + x) = make_float2(a, b);
             } else {
@@ -395,6 +407,7 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS)
                 if (x + 1 < d) dst[x + 1] = b;
             }
         }
+        bad[half] = odd != 0.f;
     }
     // Rows with a non-finite value again, by their definition, after the
     // warp's own stores above.  A row is shared by four lanes.
