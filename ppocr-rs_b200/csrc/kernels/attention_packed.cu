@@ -15,7 +15,9 @@
 // then for its tiles, and computes for a short while, so what counts is how
 // many blocks an SM holds.  256 lines of 20 to 160 tokens, 8 heads of 24
 // (35 MB, 5.4 us at the copy rate): 45.7 us with six blocks per SM, 48.9 with
-// five, 57.9 with eight (registers spilled).
+// five, 57.9 with eight (registers spilled).  The issue slots are then 70 % busy, so
+// instructions count next: with the scale in the exponent's multiply-add, masks only
+// where a tile needs them and 32-bit divisions and strides, 41.6 us.
 #include "attention_packed.cuh"
 
 namespace ppocr {
@@ -255,13 +257,16 @@ cudaError_t launch_dp(const PackedAttentionParams& p, cudaStream_t stream) {
 cudaError_t launch_attention_packed(const PackedAttentionParams& p, cudaStream_t stream) {
     if (p.total_q == 0 || p.sequences == 0) return cudaSuccess;
     if (p.dtype == DT_F32) return launch_attention_packed_f32(p, stream);
-    // tcgen05 from 16,384 keys x (padded) values per sequence on.  Measured on
-    // 16,384 tokens in causal sequences of equal length, mma.sync / tcgen05 in us:
-    //   8 heads of 24          length 384: 44 / 57, 512: 53 / 55, 1,024: 89 / 67
-    //   16 of 64, 4 KV heads   length 128: 62 / 72, 192: 72 / 73, 256: 83 / 74
-    //   8 of 128               length 96: 95 / 83, 128: 82 / 68, 512: 150 / 64
+    // tcgen05 from 16,384 keys x (padded) values per sequence on, 24,576 where its
+    // 64 values to a row are half empty.  Measured on 16,384 tokens in causal
+    // sequences of equal length, mma.sync / tcgen05 in us:
+    //   8 heads of 24           length 384: 38 / 57, 512: 47 / 55, 1,024: 78 / 67
+    //   16 of 64, 4 KV heads    length 128: 64 / 72, 192: 74 / 73, 256: 85 / 74
+    //   8 of 128                length 96: 78 / 84, 128: 67 / 68, 512: 131 / 64
+    //   32 of 128, 8 KV heads   length 64: 216 / 171, 128: 252 / 158
     const int padded = p.d <= 16 ? 16 : p.d <= 32 ? 32 : p.d <= 64 ? 64 : 128;
-    if ((long long)p.total_k * padded >= 16384ll * p.sequences && attention_tc_supported(p)) return launch_attention_tc(p, stream);
+    const long long least = padded <= 32 ? 24576 : 16384;
+    if ((long long)p.total_k * padded >= least * p.sequences && attention_tc_supported(p)) return launch_attention_tc(p, stream);
     if (p.d <= 16) return launch_dp<16>(p, stream);
     if (p.d <= 32) return launch_dp<32>(p, stream);
     if (p.d <= 64) return launch_dp<64>(p, stream);

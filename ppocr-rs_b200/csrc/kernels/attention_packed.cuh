@@ -14,12 +14,17 @@ template <typename T>
 __device__ __noinline__ void attend_row(const T* q, const T* k, long long k_stride, const T* v, long long v_stride, int d,
                                         int keys, float scale_log2, T* out) {
     const int lane = threadIdx.x & 31;
+    // Both passes compute a score in the same steps: where its rounding is worth
+    // more than a power of two, the largest one's weight is 1 all the same.
+    auto score = [&](int j) {
+        float s = 0.f;
+        for (int x = 0; x < d; ++x) s = fmaf(to_f(q[x]), to_f(k[j * k_stride + x]), s);
+        return __fmul_rn(s, scale_log2);
+    };
     float top = -INFINITY;
     bool nan = false;
     for (int j = lane; j < keys; j += 32) {
-        float s = 0.f;
-        for (int x = 0; x < d; ++x) s = fmaf(to_f(q[x]), to_f(k[j * k_stride + x]), s);
-        s *= scale_log2;
+        const float s = score(j);
         nan |= isnan(s);
         top = fmaxf(top, s);
     }
@@ -28,16 +33,15 @@ __device__ __noinline__ void attend_row(const T* q, const T* k, long long k_stri
     nan = __any_sync(0xffffffffu, nan) || top == INFINITY;
     float acc[kPackedMaxD / 32] = {}, sum = 0.f;
     if (!nan && top != -INFINITY) {
-        for (int j = 0; j < keys; ++j) {
-            float s = 0.f;
-            for (int x = lane; x < d; x += 32) s = fmaf(to_f(q[x]), to_f(k[j * k_stride + x]), s);
+        for (int j0 = 0; j0 < keys; j0 += 32) {
+            const float w = j0 + lane < keys ? exp2_hw(score(j0 + lane) - top) : 0.f;
+            for (int j = j0; j < min(j0 + 32, keys); ++j) {
+                const float wj = __shfl_sync(0xffffffffu, w, j - j0);
+                sum += wj;
 #pragma unroll
-            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            const float w = exp2_hw(s * scale_log2 - top);
-            sum += w;
-#pragma unroll
-            for (int i = 0; i < kPackedMaxD / 32; ++i)
-                if (lane + 32 * i < d) acc[i] = fmaf(w, to_f(v[j * v_stride + lane + 32 * i]), acc[i]);
+                for (int i = 0; i < kPackedMaxD / 32; ++i)
+                    if (lane + 32 * i < d) acc[i] = fmaf(wj, to_f(v[j * v_stride + lane + 32 * i]), acc[i]);
+            }
         }
     }
 #pragma unroll

@@ -24,7 +24,7 @@
 // every 4 where it stood between two barriers; with eight warps one half of
 // them splits the next tile while the other half multiplies (95 -> 89 us).
 // Chunks of 3 requests, 16 heads of 64, 4 KV heads: 78 us (TF32 pieces split by
-// each warp: 165).  64 lines of 4 to 200 tokens, 8 heads of 15: 30 us, latency.
+// each warp: 165).  64 lines of 4 to 200 tokens, 8 heads of 15: 27 us, latency.
 //
 // Softmax: weights are relative to a maximum that moves only when a score passes
 // it by more than 4 (in log2), so most tiles need no reduction; likewise the

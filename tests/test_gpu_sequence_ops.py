@@ -148,6 +148,33 @@ def test_packed_long_groups(gpu, heads, kv, causal):
     run_packed(gpu, [257, 1, 300], [400, 500, 300], heads, kv, 64, "bf16", causal, seed=heads)
 
 
+@pytest.mark.parametrize("d", [8, 16, 24, 32])
+@pytest.mark.parametrize("n", [767, 1700])
+def test_packed_small_heads_on_both_sides_of_the_rule(gpu, d, n):
+    run_packed(gpu, [n], [n], 2, 1, d, "bf16", True, seed=n + d)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [40, 700])
+@pytest.mark.parametrize("d", [16, 64])
+@pytest.mark.parametrize("size", [1e5, 1e12, 1e18, 3e19])
+def test_packed_scores_beyond_fp32(gpu, n, size, d, dtype):
+    """Products near and past FP32's range: rows whose largest score is finite take that key's value (the next
+    score is far below), rows whose score overflows are no numbers."""
+    q = torch.full((n, 1, d), size, device="cuda").to(DT[dtype])
+    k = torch.zeros(n, 1, d, device="cuda").to(DT[dtype])
+    k[:, 0, 0] = torch.linspace(0.1, 1, n, device="cuda").to(DT[dtype]) * size
+    k[n // 2, 0, 0] = 4 * size
+    v = torch.randn(n, 1, d, device="cuda", generator=rng(n)).to(DT[dtype])
+    out = torch.empty_like(q)
+    gpu.attention_packed(q, k, v, offsets([n]), offsets([n]), out, scale=1.0, stream=torch.cuda.current_stream())
+    gpu.synchronize(torch.cuda.current_stream())
+    if 4 * size * size * 1.45 < 3e38:
+        assert torch.allclose(out.float(), v[n // 2].float().expand(n, 1, d), rtol=2.0 ** -6)
+    else:
+        assert torch.isnan(out).all()
+
+
 @pytest.mark.parametrize("d", [1, 15, 16, 31, 32, 33, 64, 72, 127, 128])
 @pytest.mark.parametrize("causal", [False, True])
 def test_packed_long_fp32(gpu, d, causal):
