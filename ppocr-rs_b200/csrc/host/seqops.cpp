@@ -263,7 +263,8 @@ int ppocr_logit_rules(ppocr_gpu* gpu, const ppocr_logit_rules_args* args, void* 
         const ppocr_logit_rules_args& a = *args;
         LogitRulesParams p;
         p.dtype = dtype_of(a.dtype);
-        require(a.rows >= 0 && a.vocab >= 0 && a.vocab <= INT_MAX - 65536, "rows and vocab must not be negative");
+        count_of(a.rows, "rows is negative or near 2^31");
+        count_of(a.vocab, "vocab is negative or near 2^31");
         const bool some = a.rows > 0 && a.vocab > 0;
         require(!some || (a.logits && a.out), "logits or out pointer is null");
         require(aligned(a.logits, dtype_size(p.dtype)) && aligned(a.out, dtype_size(p.dtype)), "logits or out is not aligned to its type");

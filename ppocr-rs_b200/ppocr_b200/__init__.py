@@ -145,10 +145,18 @@ class _LoadOptions(C.Structure):
 _TOKENS = "Pqq"
 _CACHE = "PPPPiiii"
 _TABLE = "Pqii"
-_ATTENTION_PACKED = struct.Struct("@iiiiifqqq" + 4 * _TOKENS + "PP").pack
-_CACHE_TOKENS = struct.Struct("@iq" + _CACHE + _TABLE + 2 * _TOKENS + "PP").pack   # append and read
-_ATTENTION_CACHED = struct.Struct("@iif4x" + _CACHE + _TABLE + 2 * _TOKENS + "P").pack
-_LOGIT_RULES = struct.Struct("@iiiiPPqqPPqPPPPPqP").pack
+class _Fields(struct.Struct):
+    def pack(self, *fields):
+        try:
+            return super().pack(*fields)
+        except (struct.error, OverflowError) as e:   # a size beyond its field, a scale beyond FP32
+            raise InvalidInput(f"invalid input: a size or number is out of range ({e})") from None
+
+
+_ATTENTION_PACKED = _Fields("@iiiiifqqq" + 4 * _TOKENS + "PP").pack
+_CACHE_TOKENS = _Fields("@iq" + _CACHE + _TABLE + 2 * _TOKENS + "PP").pack   # append and read
+_ATTENTION_CACHED = _Fields("@iif4x" + _CACHE + _TABLE + 2 * _TOKENS + "P").pack
+_LOGIT_RULES = _Fields("@iiiiPPqqPPqPPPPPqP").pack
 
 
 _SIZE4 = C.c_size_t * 4

@@ -160,6 +160,22 @@ def test_other_refusals(gpu, call, change, words):
 
 
 @pytest.mark.parametrize("call,change", [
+    (packed, dict(scale=1e39)), (packed, dict(scale=1e31)), (cached, dict(scale=1e300)),
+    (packed, dict(q_offsets=arr(((1 << 31) + 1,), "i32"), k_offsets=arr(((1 << 31) + 1,), "i32"))),
+    (packed, dict(q=arr((1 << 31, 4, 16)), out=arr((1 << 31, 4, 16)))),
+    (packed, dict(q=arr((10, 1 << 33, 16)), out=arr((10, 1 << 33, 16)))),
+    (cached, dict(table=arr((3, 1 << 33), "i32"))),
+    (append, dict(k=arr((1 << 31, 2, 16)), v=arr((1 << 31, 2, 16)))),
+    (rules, dict(logits=arr((4, 1 << 31)), out=arr((4, 1 << 31)))),
+    (rules, dict(logits=arr(((1 << 31) - 1, 1)), out=arr(((1 << 31) - 1, 1)))),
+    (rules, dict(logits=arr((1 << 40, 1)), out=arr((1 << 40, 1)))),
+])
+def test_sizes_and_scales_out_of_range_are_refused(gpu, call, change):
+    with pytest.raises(P.InvalidInput):
+        call(gpu, **change)
+
+
+@pytest.mark.parametrize("call,change", [
     (packed, dict(q_offsets=arr((3,), "i32", ptr=A + 2))), (packed, dict(k_offsets=arr((3,), "i32", ptr=A + 1))),
     (cached, dict(lengths=arr((3,), "i32", ptr=A + 2))), (cached, dict(table=arr((3, 2), "i32", ptr=A + 2))),
     (append, dict(offsets=arr((4,), "i32", ptr=A + 1))), (append, dict(held=arr((3,), "i32", ptr=A + 2))),
