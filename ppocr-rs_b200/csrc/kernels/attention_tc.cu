@@ -49,20 +49,22 @@ constexpr int kEmulated = 2;   // of every eight pairs of exponentials, on the F
 
 // 2^x of two values, x <= 2^20, without the special function unit: x = n + f
 // with n the nearest integer (by adding 1.5 x 2^23, whose last mantissa bit is
-// 1), 2^f by the polynomial of degree 4 with the least largest relative error
-// on [-1/2, 1/2] (2.6e-6, a thousandth of the BF16 rounding that follows), and
-// n added to the exponent.  Below 2^-126 it gives about that.
+// 1), 2^f by the polynomial of degree 4 that is 1 at 0 with the least largest
+// relative error on [-1/2, 1/2] (2.9e-6, a thousandth of the BF16 rounding that
+// follows), and n added to the exponent.  From -127 down, -infinity (a masked
+// score) among them, f is 0 and the exponent field of 1 less 127 leaves exactly
+// 0; in between the result is some number below 2^-126.
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));   // -126; a NaN stays one
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));   // -127; a NaN stays one
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
     const float2 magic = make_float2(12582912.f, 12582912.f);
     const float2 t = __fadd2_rn(x, magic);
     const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
     const float2 f = __fadd2_rn(x, make_float2(-n.x, -n.y));
-    float2 y = __ffma2_rn(f, make_float2(0.0095701f, 0.0095701f), make_float2(0.05591786f, 0.05591786f));
-    y = __ffma2_rn(y, f, make_float2(0.24024745f, 0.24024745f));
-    y = __ffma2_rn(y, f, make_float2(0.69312181f, 0.69312181f));
-    y = __ffma2_rn(y, f, make_float2(0.99999926f, 0.99999926f));
+    float2 y = __ffma2_rn(f, make_float2(0.009585382f, 0.009585382f), make_float2(0.05590663f, 0.05590663f));
+    y = __ffma2_rn(y, f, make_float2(0.24024038f, 0.24024038f));
+    y = __ffma2_rn(y, f, make_float2(0.6931242f, 0.6931242f));
+    y = __ffma2_rn(y, f, make_float2(1.f, 1.f));
     return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)),
                        __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
 }
@@ -437,9 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         }
         if (ok && tiles > 0) wait(&o_full[t], 0, 6);
         if (ok && live) {
-            // top: -infinity where every score is (or is no number), and then the
-            // emulated weights are not quite 0.
-            const float inv = sum == 0.f || (top == -INFINITY && !isnan(sum)) ? 0.f : 1.f / sum;
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const int token = w.qs.begin + w.token0 + t * w.per + row / w.group, head = w.kv * w.group + row % w.group;
             __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out.ptr) + token * p.out.token_stride + head * p.out.head_stride;
             bool bad = false;

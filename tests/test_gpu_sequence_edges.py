@@ -1,0 +1,78 @@
+"""Sequence operators at the ends of their ranges, against plain float64 implementations.
+
+Tolerances are those of the sequence operators' other tests, the sums of the roundings that the kernels document;
+what a test adds to them stands beside it.
+"""
+
+import math
+
+import pytest
+
+import ppocr_b200 as P
+
+torch = pytest.importorskip("torch")
+import test_gpu_sequence_ops as ops  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+DT, HALF_STEP = ops.DT, ops.HALF_STEP
+
+
+def packed(gpu, q, k, v, nq, nk, causal=False, scale=None):
+    s = torch.cuda.current_stream()
+    out = torch.full_like(q, 7.0)
+    gpu.attention_packed(q, k, v, ops.offsets(nq), ops.offsets(nk), out, causal=causal, scale=scale, stream=s)
+    gpu.synchronize(s)
+    return out
+
+
+# ---------------------------------------------------------------------------
+# Packed attention: masked keys and values, whatever they hold
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [24, 64, 128])
+@pytest.mark.parametrize("n", [100, 1000])
+@pytest.mark.parametrize("causal", [False, True])
+def test_packed_masked_finite_values_change_no_bit(gpu, n, d, causal, dtype):
+    """Large finite values behind a row's last key, and keys and values in the sequence between and behind the last
+    one."""
+    g = ops.rng(n + d)
+    lengths, behind = [n, n - 3, n], 150
+    q, k, v = (torch.randn(sum(lengths) + behind, h, d, device="cuda", generator=g).to(DT[dtype]) for h in (4, 2, 2))
+    masked = torch.zeros(q.shape[0], dtype=torch.bool, device="cuda")
+    masked[n:2 * n - 3] = True                     # all of the middle sequence
+    masked[sum(lengths):] = True
+    others, rows = masked.clone(), ~masked
+    if causal:                                     # the last values of the first sequence: seen by its last queries
+        masked[n - 3:n] = True
+        rows[n - 3:n] = False
+    huge = torch.where(torch.rand(v.shape, device="cuda", generator=g) < 0.5, 3e38, -3e38).to(DT[dtype])
+    outs = []
+    for fill in (torch.zeros_like(huge), huge):
+        kk, vv = k.clone(), v.clone()
+        kk[others], vv[masked] = fill[others], fill[masked]
+        outs.append(packed(gpu, q, kk, vv, lengths, lengths, causal))
+    assert torch.isfinite(outs[0][rows]).all()
+    assert torch.equal(outs[0][rows], outs[1][rows])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [40, 1000])
+@pytest.mark.parametrize("below", [160, 300, 100000])
+def test_packed_keys_far_below_weigh_nothing(gpu, n, below, dtype):
+    """Visible keys whose scores lie `below` powers of two under the others' have no weight, however large their
+    values (2^-160 of 1e38 is 1e-10)."""
+    d = 64
+    g = ops.rng(n)
+    q, k, v = (torch.randn(n, 2, d, device="cuda", generator=g) for _ in range(3))
+    q[..., 0] = 1.0
+    k[..., 0] = 0.0
+    far = torch.rand(n, device="cuda", generator=g) < 0.5
+    far[n // 3] = False
+    k[far, :, 0] = -float(below) * 8 * math.log(2) * 1.1   # scale 1 / 8; the other products stay within a tenth
+    v[far] = 1e38
+    q, k, v = (x.to(DT[dtype]) for x in (q, k, v))
+    out = packed(gpu, q, k, v, [n], [n])
+    ref, mag, prod = ops.attend(q.double(), k[~far].double(), v[~far].double(), d ** -0.5)
+    ops.check(out, ref, ops.tolerance(ref, mag, prod, d, n, dtype, 2.0 ** -8 if dtype == "bf16" else 2.0 ** -20) + 1e-9)
