@@ -218,10 +218,11 @@ __global__ void __launch_bounds__(kReadThreads) cache_read_kernel(CacheReadParam
     for (int i = threadIdx.x / 32; i < tokens; i += kReadThreads / 32) {
         const int t = t0 + i, seq = find_owner(p.table.sequences, t, [&](int s) { return seq_offset(p.offsets, 0, s, p.total); });
         // Sequences without tokens start where the next one does: the last one is the owner.
-        const int begin = p.offsets[seq], end = p.offsets[seq + 1], first = p.first[seq];
+        const Span span = seq_span(p.offsets, 0, seq, p.total, p.bad);
+        const int first = p.first[seq];
         int w = -1, at = 0;
-        if (t >= begin && t < end) {
-            const long long pos = (long long)first + (t - begin);
+        if (t >= span.begin && t - span.begin < span.len) {
+            const long long pos = (long long)first + (t - span.begin);
             if (first >= 0 && pos < (long long)p.table.width * p.cache.page) {
                 w = p.table.pages[seq * p.table.stride + pos / p.cache.page];
                 at = (int)(pos % p.cache.page);

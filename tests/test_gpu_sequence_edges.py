@@ -76,3 +76,39 @@ def test_packed_keys_far_below_weigh_nothing(gpu, n, below, dtype):
     out = packed(gpu, q, k, v, [n], [n])
     ref, mag, prod = ops.attend(q.double(), k[~far].double(), v[~far].double(), d ** -0.5)
     ops.check(out, ref, ops.tolerance(ref, mag, prod, d, n, dtype, 2.0 ** -8 if dtype == "bf16" else 2.0 ** -20) + 1e-9)
+
+
+# ---------------------------------------------------------------------------
+# Bad offsets
+# ---------------------------------------------------------------------------
+
+def read_by_hand(cache, table, offsets, first, total, page, kv, d):
+    """What a read may write: each token by the sequence whose clamped offsets hold it, None elsewhere."""
+    k = [None] * total
+    for i in range(len(offsets) - 1):
+        a = min(max(offsets[i], 0), total)
+        b = min(max(offsets[i + 1], a), total)
+        for t in range(a, b):
+            pos = first[i] + t - a
+            k[t] = cache.k[table[i, pos // page].long(), :, pos % page].float() * cache.k_scales[table[i, pos // page].long()][:, None]
+    return k
+
+
+@pytest.mark.parametrize("bad", [[-4, 10, 20], [0, 10, 25], [-2 ** 31, 10, 20], [0, 2 ** 31 - 1, 20], [-2 ** 31, 2 ** 31 - 1, 20],
+                                 [0, 10, -2 ** 31], [5, 3, 20]])
+def test_read_clamps_and_reports_bad_offsets(gpu, bad):
+    """A token of the output is what the clamped offsets say, or left as it was; the next synchronize reports them."""
+    g = ops.rng(3)
+    page, kv, d, total = 16, 2, 16, 20
+    cache, table = ops.make_cache(g, [60, 60], kv, d, page)
+    first = [3, 7]
+    s = torch.cuda.current_stream()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    k, v = (torch.full((total, kv, d), 7.0, device="cuda") for _ in range(2))
+    gpu.cache_read(cache, k, v, torch.tensor(bad, **i32), torch.tensor(first, **i32), table, stream=s)
+    with pytest.raises(P.InvalidInput, match="out of range"):
+        gpu.synchronize(s)
+    want = read_by_hand(cache, table, bad, first, total, page, kv, d)
+    for t in range(total):
+        same = want[t] is not None and torch.equal(k[t], want[t])
+        assert same or ((k[t] == 7).all() and (v[t] == 7).all()), t
