@@ -62,6 +62,10 @@ struct PackedPiece {
         group = p.heads / p.kv_heads;
         kv = blockIdx.x % p.kv_heads;
         causal = p.causal;
+        if ((long long)blockIdx.x * blockDim.x < p.sequences) {
+            check_offsets(p.q_offsets, p.sequences, p.total_q, p.bad);
+            check_offsets(p.k_offsets, p.sequences, p.total_k, p.bad);
+        }
         // The longest rows of a causal sequence are dealt first.
         const long long pieces = gridDim.x / p.kv_heads, at_id = blockIdx.x / p.kv_heads;
         const long long id = causal ? pieces - 1 - at_id : at_id;

@@ -208,6 +208,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
     Work w;
+    check_offsets(p.q_offsets, p.sequences, p.total_q, p.bad);
+    check_offsets(p.k_offsets, p.sequences, p.total_k, p.bad);
     if (!find_work(p, w)) return;   // the whole CTA
     uint8_t* smem = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* sq = smem;

@@ -92,6 +92,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 8 : 7) cache_append
     // A sequence's n new tokens touch at most n / page + 2 pages.
     const int page = p.cache.page, d8 = p.cache.d / 8;
     const int page_shift = 31 - __clz(page), id = blockIdx.x;
+    check_offsets(p.offsets, p.table.sequences, p.total, p.bad);
     auto first_id = [&](int i) { return (seq_offset(p.offsets, 0, i, p.total) >> page_shift) + 2 * i; };
     const int seq = find_owner(p.table.sequences, id, first_id);
     const int index = id - first_id(seq);   // of the pages this sequence's new tokens touch
@@ -215,6 +216,7 @@ __global__ void __launch_bounds__(kReadThreads) cache_read_kernel(CacheReadParam
     __shared__ int where[kReadTokens], slot[kReadTokens];
     const int t0 = blockIdx.x * kReadTokens, lane = threadIdx.x & 31;
     const int tokens = min(kReadTokens, p.total - t0);
+    check_offsets(p.offsets, p.table.sequences, p.total, p.bad);
     for (int i = threadIdx.x / 32; i < tokens; i += kReadThreads / 32) {
         const int t = t0 + i, seq = find_owner(p.table.sequences, t, [&](int s) { return seq_offset(p.offsets, 0, s, p.total); });
         // Sequences without tokens start where the next one does: the last one is the owner.

@@ -25,6 +25,17 @@ __device__ __forceinline__ Span seq_span(const int32_t* offsets, int uniform, in
     return Span{cb, min(max(e, cb), total) - cb};
 }
 
+// Reports bad offsets of any sequence: with offsets that fall inside a longer
+// list, find_owner passes over sequences, whose blocks then look at no offset.
+// The grid's first blocks take the sequences by turns; nothing waits for it.
+__device__ __forceinline__ void check_offsets(const int32_t* offsets, int sequences, int total, int* bad) {
+    if ((long long)blockIdx.x * blockDim.x >= sequences || (blockIdx.y | blockIdx.z) != 0 || !offsets) return;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < sequences; i += (long long)gridDim.x * blockDim.x) {
+        const int b = __ldg(offsets + i), e = __ldg(offsets + i + 1);
+        if (b < 0 || e < b || e > total) seq_bad_index(bad);
+    }
+}
+
 // Deals ids to the sequences without a prefix sum: sequence i owns the ids
 // [first(i), first(i + 1)), where first() needs i's offset alone and grows with
 // i by at least i's number of pieces (some ids then own no piece).  A converged

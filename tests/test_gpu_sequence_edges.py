@@ -112,3 +112,34 @@ def test_read_clamps_and_reports_bad_offsets(gpu, bad):
     for t in range(total):
         same = want[t] is not None and torch.equal(k[t], want[t])
         assert same or ((k[t] == 7).all() and (v[t] == 7).all()), t
+
+
+BAD_OFFSETS = [[0, 3000, 100, 4000], [0, 100, 50, 120], [0, 4000, 3999, 4000, 4000], [0, 10, 4001, 20, 4000],
+               [0, 10, -1, 20, 4000], [4000, 4000, 2 ** 31 - 1], [0, 4000, 4000, -2 ** 31, 4000, 4000]]
+
+
+@pytest.mark.parametrize("bad", BAD_OFFSETS)
+def test_every_bad_offset_is_reported(gpu, bad):
+    """Also those of sequences that no block works on: offsets inside a longer list, sequences without tokens."""
+    g = ops.rng(4)
+    n, page, total = len(bad) - 1, 16, 4000
+    s = torch.cuda.current_stream()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    good = torch.tensor([0] + [total * (i + 1) // n for i in range(n)], **i32)
+    off = torch.tensor(bad, **i32)
+    cache, table = ops.make_cache(g, [total] * n, 2, 64, page)
+    zero = torch.zeros(n, **i32)
+
+    def refused(call, *args, **kw):
+        call(*args, stream=s, **kw)
+        with pytest.raises(P.InvalidInput, match="out of range"):
+            gpu.synchronize(s)
+
+    for dtype in (torch.float32, torch.bfloat16):
+        q, k, v = (torch.randn(total, 2, 64, device="cuda", generator=g).to(dtype) for _ in range(3))
+        for a, b in ((off, good), (good, off)):
+            refused(gpu.attention_packed, q, k, v, a, b, torch.empty_like(q), causal=True)
+        refused(gpu.attention_packed, q[:, :, :15], k[:, :, :15], v[:, :, :15], off, good, torch.empty_like(q)[:, :, :15])
+        refused(gpu.cache_read, cache, k, v, off, zero, table)
+        refused(gpu.cache_append, cache, k, v, off, zero, table)
+    gpu.synchronize(s)   # reported once each
