@@ -406,8 +406,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             }
             const float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * scale;
             if (__any_sync(0xffffffffu, most > top + kSlack)) {
-                const float next = fmaxf(top, most);
-                const float g = top == -INFINITY ? 0.f : exp2_hw(top - next);
+                // The warp's branch, but each row by its own scores: a key that a row
+                // must not see cannot move what its neighbour's rounding depends on.
+                const float next = most > top + kSlack ? most : top;
+                const float g = next == top ? 1.f : top == -INFINITY ? 0.f : exp2_hw(top - next);
                 top = next;
                 ref = top == -INFINITY ? 0.f : top;
                 sum *= g;

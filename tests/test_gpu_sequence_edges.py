@@ -143,3 +143,18 @@ def test_every_bad_offset_is_reported(gpu, bad):
         refused(gpu.cache_read, cache, k, v, off, zero, table)
         refused(gpu.cache_append, cache, k, v, off, zero, table)
     gpu.synchronize(s)   # reported once each
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [24, 64, 128])
+@pytest.mark.parametrize("n", [100, 1000])
+def test_packed_masked_keys_change_no_bit(gpu, n, d, dtype):
+    """Keys that only the last queries see, with scores far above the others', leave the other rows as they were."""
+    g = ops.rng(n + d)
+    q, k, v = (torch.randn(n, h, d, device="cuda", generator=g).to(DT[dtype]) for h in (4, 2, 2))
+    outs = []
+    for factor in (1, 1000):
+        kk = k.clone()
+        kk[n - 3:] *= factor
+        outs.append(packed(gpu, q, kk, v, [n], [n], True))
+    assert torch.equal(outs[0][:n - 3], outs[1][:n - 3])
