@@ -9,7 +9,7 @@
 // registers; scores and weights never leave them.  Weights are rounded to BF16
 // for the second product (2^-8 of a weight at most, averaged over the keys; the
 // sum uses the unrounded ones).  Rows with no key give zeros; a non-finite row
-// is computed again from its definition (attend_row).
+// and one of scores beyond 2^24 is computed again from its definition (attend_row).
 //
 // Short lines are bound by latency: a block waits for its sequence's offsets,
 // then for its tiles, and computes for a short while, so what counts is how
@@ -201,7 +201,6 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 6)
     l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    // A maximum whose scaled value overflows leaves sums of 0 or NaN: no number, so the row is computed again.
     const float i0 = m0 == -INFINITY ? 0.f : 1.f / l0, i1 = m1 == -INFINITY ? 0.f : 1.f / l1;
     T* out = at.queries<T>(p.out);
     bool bad[2] = {false, false};
@@ -224,10 +223,10 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 3 : DP > 32 ? 4 : 6)
                 if (x + 1 < d) dst[x + 1] = from_f<T>(b);
             }
         }
-        bad[half] = odd != 0.f;
+        bad[half] = odd != 0.f || rounding_spoils((half ? m1 : m0) * scale);
     }
-    // Rows with a non-finite value again, by their definition, after the
-    // warp's own stores above.  A row is shared by four lanes.
+    // Rows with a non-finite value or too large scores again, by their definition,
+    // after the warp's own stores above.  A row is shared by four lanes.
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         const unsigned again = __ballot_sync(0xffffffffu, bad[half]);

@@ -9,7 +9,8 @@ namespace ppocr {
 // One row, one warp, from its definition: no key past `keys` is read.  The
 // tiled kernels multiply the zero weights of masked keys with those keys'
 // values, so an infinity or NaN among masked values of a tile spoils rows that
-// must not see it; a row that came out non-finite is computed again here.
+// must not see it; a row that came out non-finite is computed again here, and so
+// is one whose scores are too large for its kernel's weights.
 template <typename T>
 __device__ __noinline__ void attend_row(const T* q, const T* k, long long k_stride, const T* v, long long v_stride, int d,
                                         int keys, float scale_log2, T* out) {
@@ -48,6 +49,13 @@ __device__ __noinline__ void attend_row(const T* q, const T* k, long long k_stri
     for (int i = 0; i < kPackedMaxD / 32; ++i)
         if (lane + 32 * i < d) out[lane + 32 * i] = from_f<T>(nan ? NAN : sum == 0.f ? 0.f : acc[i] / sum);
 }
+
+// Kernels that take the scale in the exponent's multiply-add hold weights relative
+// to the rounded product of largest score and scale, so a row's weights share a
+// factor of 2^(that rounding's error).  Up to a product of 2^24 it is at most 2^1;
+// near 2^31 it can pass FP32's range either way, where a finite result may be
+// wrong.  Rows beyond 2^24 are computed again from their definition.
+__device__ __forceinline__ bool rounding_spoils(float top) { return top != -INFINITY && fabsf(top) > 16777216.f; }
 
 // A block's piece of the mma.sync kernels: up to ROWS rows (row = query token x
 // group + head) of one (sequence, KV head).

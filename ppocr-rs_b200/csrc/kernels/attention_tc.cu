@@ -28,7 +28,8 @@
 //
 // Every wait is bounded: on expiry the CTA records a code in *err, stops,
 // lets its copies and MMAs land, frees its TMEM and returns.  Rows that come
-// out non-finite are computed again from their definition (attend_row).
+// out non-finite and those of scores beyond 2^24 are computed again from their
+// definition (attend_row).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -47,7 +48,7 @@ constexpr int kTmemCols = 512;
 constexpr float kSlack = 8.f;
 constexpr int kEmulated = 2;   // of every eight pairs of exponentials, on the FMA pipes (0: 263 us, 1: 256, 2: 257, 3: 279)
 
-// 2^x of two values, x <= 2^20, without the special function unit: x = n + f
+// 2^x of two values, x < 127, without the special function unit: x = n + f
 // with n the nearest integer (by adding 1.5 x 2^23, whose last mantissa bit is
 // 1), 2^f by the polynomial of degree 4 that is 1 at 0 with the least largest
 // relative error on [-1/2, 1/2] (2.9e-6, a thousandth of the BF16 rounding that
@@ -446,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const int token = w.qs.begin + w.token0 + t * w.per + row / w.group, head = w.kv * w.group + row % w.group;
             __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out.ptr) + token * p.out.token_stride + head * p.out.head_stride;
-            bool bad = false;
+            bool bad = row < live && rounding_spoils(top);
             // Straight from TMEM, a row per lane.  (Through shared memory, with 512
             // bytes to a store, it took 5,000 cycles instead of 3,000: the other
             // tile's scores keep shared memory busy.)

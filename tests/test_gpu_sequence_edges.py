@@ -158,3 +158,46 @@ def test_packed_masked_keys_change_no_bit(gpu, n, d, dtype):
         kk[n - 3:] *= factor
         outs.append(packed(gpu, q, kk, v, [n], [n], True))
     assert torch.equal(outs[0][:n - 3], outs[1][:n - 3])
+
+
+# ---------------------------------------------------------------------------
+# Packed attention: scores beyond what FP32 resolves
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [16, 64, 128])
+@pytest.mark.parametrize("n,at", [(40, 5), (40, 17), (700, 0), (700, 334), (700, 339), (700, 350), (700, 699)])
+@pytest.mark.parametrize("power", [20, 28, 32, 36, 44, 70])
+def test_packed_scores_far_beyond_their_roundings(gpu, power, n, at, d, dtype):
+    """Scores near 2^power, of either rounding, whose largest is four times the next: its key's value alone."""
+    g = ops.rng(power + at)
+    q = torch.zeros(n, 1, d, device="cuda")
+    q[:, 0, 0] = (1 + torch.rand(n, device="cuda", generator=g)) * 2.0 ** (power - power // 2)
+    k = torch.zeros(n, 1, d, device="cuda")
+    k[:, 0, 0] = torch.rand(n, device="cuda", generator=g) * 2.0 ** (power // 2)
+    k[at, 0, 0] = (1 + torch.rand(1, device="cuda", generator=g).item()) * 4 * 2.0 ** (power // 2)
+    v = torch.randn(n, 1, d, device="cuda", generator=g)
+    q, k, v = (x.to(DT[dtype]) for x in (q, k, v))
+    for scale in (1.0, 0.7, 0.9):
+        out = packed(gpu, q, k, v, [n], [n], scale=scale)
+        ref = v[at].double().expand(n, 1, d)
+        ops.check(out, ref, ref.abs() * (2 * HALF_STEP[dtype] + 2.0 ** -20) + 1e-30, f"scale {scale}")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [40, 700])
+@pytest.mark.parametrize("power", [24, 33, 40])
+def test_packed_equal_scores_far_beyond_their_roundings(gpu, power, n, dtype):
+    """The same key at several places, far above the others: the mean of its values."""
+    d, at = 64, [1, 6, 13, 30, n - 1]
+    g = ops.rng(power + n)
+    q, k = torch.zeros(n, 1, d, device="cuda"), torch.zeros(n, 1, d, device="cuda")
+    q[:, 0, 3] = (1 + torch.rand(n, device="cuda", generator=g)) * 2.0 ** power
+    k[:, 0, 3] = torch.rand(n, device="cuda", generator=g)
+    k[at, 0, 3] = 4.7
+    v = torch.randn(n, 1, d, device="cuda", generator=g)
+    q, k, v = (x.to(DT[dtype]) for x in (q, k, v))
+    for scale in (1.0, 0.7, 0.9):
+        out = packed(gpu, q, k, v, [n], [n], scale=scale)
+        ref, mag = v[at].double().mean(0).expand(n, 1, d), v[at].double().abs().mean(0).expand(n, 1, d)
+        ops.check(out, ref, HALF_STEP[dtype] * ref.abs() + mag * (HALF_STEP[dtype] + 2.0 ** -20) + 1e-30, f"scale {scale}")
