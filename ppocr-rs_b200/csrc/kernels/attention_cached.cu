@@ -50,6 +50,7 @@ constexpr int kWarps = 4, kThreads = 32 * kWarps, kHeads = 8, kMaxSplits = 16;
 constexpr int kTile = 16;             // tokens per tile: within one page, whatever its size
 constexpr int kPair = 2;              // tiles that a warp takes at a time: two independent chains of products
 constexpr float kSlack = 8.f;         // log2 of the largest weight before the maximum moves
+constexpr float kLeastRef = 0x1p-120f;   // of R, so that what it divides stays finite
 constexpr float kWeightScale = 64.f;  // weights are held times 64: a larger range above FP16's subnormals
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
@@ -343,12 +344,12 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
                 n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
             }
             const float g0 = m0 == -INFINITY ? 0.f : exp2_hw(m0 - n0), g1 = m1 == -INFINITY ? 0.f : exp2_hw(m1 - n1);
-            const float next = fmaxf(ref, tv);
+            const float next = fmaxf(fmaxf(ref, tv), kLeastRef);
             const float back = next > ref ? ref / next : 1.f;
             m0 = n0; m1 = n1; ref = next;
             b0 = m0 == -INFINITY ? 0.f : m0;
             b1 = m1 == -INFINITY ? 0.f : m1;
-            unit = ref > 0.f ? kWeightScale / ref : 1.f;   // 0 only while every V scale seen is 0: weights of zeros
+            unit = kWeightScale / ref;
             l0 *= g0; l1 *= g1;
 #pragma unroll
             for (int j = 0; j < KS; ++j) {

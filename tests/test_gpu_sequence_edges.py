@@ -201,3 +201,53 @@ def test_packed_equal_scores_far_beyond_their_roundings(gpu, power, n, dtype):
         out = packed(gpu, q, k, v, [n], [n], scale=scale)
         ref, mag = v[at].double().mean(0).expand(n, 1, d), v[at].double().abs().mean(0).expand(n, 1, d)
         ops.check(out, ref, HALF_STEP[dtype] * ref.abs() + mag * (HALF_STEP[dtype] + 2.0 ** -20) + 1e-30, f"scale {scale}")
+
+
+# ---------------------------------------------------------------------------
+# Single-token attention: pages whose values lie far apart
+# ---------------------------------------------------------------------------
+
+def check_cached_relative(out, q, cache, table, lengths, page, dtype):
+    """As the other tests' check, but what a small weight may lose is counted relative to the largest product of a
+    weight and its V scale: 2^-31 for the one FP16 piece of BF16 calls, 2^-41 for the two of FP32 ones; 2^-133 and
+    2^-147 are steps of the smallest numbers."""
+    d = q.shape[-1]
+    for i, n in enumerate(lengths):
+        k, v = ops.cache_values(cache, table, i, n, page)
+        ref, mag, prod = ops.attend(q[i:i + 1].double(), k, v, d ** -0.5)
+        tol = ops.tolerance(ref, mag, prod, d, n, dtype, 2.0 ** -11 if dtype == "bf16" else 2.0 ** -20) - 1e-30
+        rows = table[i, : -(-n // page)].long()
+        scales = cache.v_scales[rows].double().repeat_interleave(page, 0)[:n, :, None].expand(-1, -1, d)
+        group, heads = q.shape[1] // k.shape[1], []
+        for h in range(q.shape[1]):
+            w = torch.softmax(k[:, h // group] @ q[i, h].double() * d ** -0.5, 0)
+            heads.append((w * scales[:, h // group, 0]).amax())
+        most = torch.stack(heads)
+        floor = n * 127 * most * (2.0 ** -31 if dtype == "bf16" else 2.0 ** -41)
+        tol = tol + floor[None, :, None] + (2.0 ** -133 if dtype == "bf16" else 2.0 ** -147) + n * 2.0 ** -143
+        ops.check(out[i:i + 1], ref, tol, f"sequence {i}, length {n}")
+
+
+def cached(gpu, cache, q, lengths, table):
+    s = torch.cuda.current_stream()
+    out = torch.full_like(q, 7.0)
+    gpu.attention_cached(cache, q, torch.tensor(lengths, dtype=torch.int32, device="cuda"), table, out, stream=s)
+    gpu.synchronize(s)
+    return out
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [24, 64, 128])
+@pytest.mark.parametrize("small", [1e-45, 1e-42, 1e-38, 1e-37, 1e-34, 1e-30])
+def test_cached_small_value_scales(gpu, small, d, dtype):
+    """Pages of the smallest values, alone and ahead of ordinary ones."""
+    g = ops.rng(d)
+    lengths, page = [40, 100, 333, 7], 16
+    cache, table = ops.make_cache(g, lengths, 2, d, page)
+    cache.v_scales[table[0, :3].long()] = small
+    cache.v_scales[table[1, 0].long()] = small
+    cache.v_scales[table[2, :20].long()] = small
+    cache.v_scales[table[3, 0].long()] = small
+    q = torch.randn(4, 4, d, device="cuda", generator=g).to(DT[dtype])
+    out = cached(gpu, cache, q, lengths, table)
+    check_cached_relative(out, q, cache, table, lengths, page, dtype)
