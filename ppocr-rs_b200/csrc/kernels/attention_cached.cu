@@ -13,8 +13,13 @@
 // Integers are exact in FP16.  q is scaled by a power of two per head to fit
 // FP16; FP32 inputs are carried as two FP16 pieces (22 bits), as are their
 // softmax weights, so their products are FP32-class.  A page's K scale
-// multiplies its scores; its V scale multiplies its weights, taken relative to
-// a running reference R so that they stay in FP16's range.
+// multiplies its scores; its V scale multiplies its weights, and the product is
+// taken relative to a power of two per head that follows the largest one: up
+// when a product would pass FP16's range, down with the weights when the maximum
+// moves.  So pages of large values and no weight cost the others no bits.  (A
+// power of the V scales alone does: at 2^27 between two pages the weights of the
+// smaller one had three bits left.)  The weights' second piece is held times
+// 2^11 and summed apart, which keeps 22 bits down to 2^-20 of the largest product.
 //
 // A warp owns every fourth pair of tiles of its block's token range, fetches
 // them with cp.async into a ring of its own in shared memory (two pairs; no
@@ -49,9 +54,10 @@ namespace cg = cooperative_groups;
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kHeads = 8, kMaxSplits = 16;
 constexpr int kTile = 16;             // tokens per tile: within one page, whatever its size
 constexpr int kPair = 2;              // tiles that a warp takes at a time: two independent chains of products
-constexpr float kSlack = 8.f;         // log2 of the largest weight before the maximum moves
-constexpr float kLeastRef = 0x1p-120f;   // of R, so that what it divides stays finite
-constexpr float kWeightScale = 64.f;  // weights are held times 64: a larger range above FP16's subnormals
+constexpr float kSlack = 6.f;         // log2 of what weights leave above the maximum: they are at most 1
+constexpr float kMost = 65000.f;      // of a weight x V scale x unit, in FP16
+constexpr int kLeast = -119;          // of the power that these products are relative to; 2^(7 - it) and 2^(it - 7) are numbers
+constexpr float kSecond = 2048.f;     // what second pieces are held times
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
@@ -269,9 +275,10 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
     for (int j = 0; j < KS; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    float b0 = 0.f, b1 = 0.f;        // m0 and m1, 0 where they are -infinity
-    float ref = 0.f, unit = 1.f;     // R, and what a V scale is multiplied by
+    // Weights are relative to m (once a score was seen); o holds sums of weight x V
+    // times 2^(7 - e) = unit.
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, unit0 = power(7 - kLeast), unit1 = unit0, units = unit0;   // the larger
+    int e0 = kLeast, e1 = kLeast;
 
     const uint32_t k_at = r * DP, v_at = Tiles::kRows + 2 * c * DP;
     for (; t < t_end; t += kWarps) {
@@ -329,36 +336,78 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
                 if (left <= 0) sv[h] = 0.f;   // what the stage holds is older
             }
         }
-        float t0 = -INFINITY, t1 = -INFINITY, tv = 0.f;
+        float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
         for (int h = 0; h < kPair; ++h) {
             t0 = fmaxf(t0, fmaxf(s[h][0], s[h][2]));
             t1 = fmaxf(t1, fmaxf(s[h][1], s[h][3]));
-            tv = fmaxf(tv, sv[h]);
         }
-        if (__any_sync(0xffffffffu, t0 > m0 + kSlack || t1 > m1 + kSlack || tv > 2.f * ref)) {
-            float n0 = fmaxf(t0, m0), n1 = fmaxf(t1, m1);
+        auto weigh = [&] {
+            const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) {
-                n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
-                n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
+            for (int h = 0; h < kPair; ++h) {
+                float* x = s[h];
+                x[0] = exp2_hw(x[0] - b0); x[1] = exp2_hw(x[1] - b1);
+                x[2] = exp2_hw(x[2] - b0); x[3] = exp2_hw(x[3] - b1);
+                l0 += x[0] + x[2];
+                l1 += x[1] + x[3];
             }
-            const float g0 = m0 == -INFINITY ? 0.f : exp2_hw(m0 - n0), g1 = m1 == -INFINITY ? 0.f : exp2_hw(m1 - n1);
-            const float next = fmaxf(fmaxf(ref, tv), kLeastRef);
-            const float back = next > ref ? ref / next : 1.f;
-            m0 = n0; m1 = n1; ref = next;
-            b0 = m0 == -INFINITY ? 0.f : m0;
-            b1 = m1 == -INFINITY ? 0.f : m1;
-            unit = kWeightScale / ref;
-            l0 *= g0; l1 *= g1;
+        };
+        // A new maximum, or a V scale whose product with a weight of 1 would pass FP16.
+        if (__any_sync(0xffffffffu, t0 > m0 || t1 > m1 || fmaxf(sv[0], sv[1]) * units > kMost)) {
+            auto rescale = [&](int head, float& unit, int& e, int next, float back) {
 #pragma unroll
-            for (int j = 0; j < KS; ++j) {
-                o[j][0] *= g0 * back; o[j][1] *= g1 * back;
-                o[j][2] *= g0 * back; o[j][3] *= g1 * back;
+                for (int j = 0; j < KS; ++j) {
+                    o[j][head] *= back;
+                    o[j][head + 2] *= back;
+                }
+                e = next;
+                unit = power(7 - e);
+            };
+            auto raise = [&](float t, float& m, float& l, int& e, float& unit, int head) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
+                if (t > m) {   // the whole head's eight lanes
+                    // What the sums hold shrinks with the weights, so their power may fall as far.
+                    const float fall = m - (t + kSlack);   // -infinity for the first tokens
+                    const int next = max(e + (int)fmaxf(ceilf(fall), -300.f), kLeast);
+                    rescale(head, unit, e, next, exp2_hw(fall + (float)(e - next)));
+                    l *= exp2_hw(fall);
+                    m = t + kSlack;
+                }
+            };
+            raise(t0, m0, l0, e0, unit0, 0);
+            raise(t1, m1, l1, e1, unit1, 1);
+            weigh();
+            auto cover = [&](float y, int& e, float& unit, int head) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, x));
+                // To between 2^6 and 2^7, although FP16 holds more: weights of up to 1 come
+                // without a look at them as long as the V scales stay near this one.
+                const int next = min(max(e, exponent(y) + 1), 126);
+                if (next > e) rescale(head, unit, e, next, power(max(e - next, -126)));   // what 2^-126 leaves of a sum counts for nothing
+            };
+            static_assert(kPair == 2, "the largest products of two tiles");
+            cover(fmaxf(fmaxf(s[0][0], s[0][2]) * sv[0], fmaxf(s[1][0], s[1][2]) * sv[1]), e0, unit0, 0);
+            cover(fmaxf(fmaxf(s[0][1], s[0][3]) * sv[0], fmaxf(s[1][1], s[1][3]) * sv[1]), e1, unit1, 1);
+            units = fmaxf(unit0, unit1);
+#pragma unroll
+            for (int h = 0; h < kPair; ++h) {
+                // The unit first: the V scale's product with it may pass FP32's range.
+                s[h][0] = s[h][0] * unit0 * sv[h]; s[h][1] = s[h][1] * unit1 * sv[h];
+                s[h][2] = s[h][2] * unit0 * sv[h]; s[h][3] = s[h][3] * unit1 * sv[h];
+            }
+        } else {
+            weigh();
+#pragma unroll
+            for (int h = 0; h < kPair; ++h) {
+                const float w0 = sv[h] * unit0, w1 = sv[h] * unit1;
+                s[h][0] *= w0; s[h][1] *= w1;
+                s[h][2] *= w0; s[h][3] *= w1;
             }
         }
         // Weights, as the B operand of the second product.
-        uint32_t p0[kPair], p1[kPair], e0[kPair], e1[kPair], v[kPair][4][DP / 32];
+        uint32_t p0[kPair], p1[kPair], r0[kPair], r1[kPair], v[kPair][4][DP / 32];
 #pragma unroll
         for (int h = 0; h < kPair; ++h) {
 #pragma unroll
@@ -367,28 +416,21 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
                 read_words<PV>(at + h * Tiles::kOne + v_at + row * DP + Tiles::v_chunk(2 * c, r * PV >> 4) * 16 + (r * PV & 15),
                                v[h][i]);
             }
-            float* x = s[h];
-            x[0] = exp2_hw(x[0] - b0); x[1] = exp2_hw(x[1] - b1);
-            x[2] = exp2_hw(x[2] - b0); x[3] = exp2_hw(x[3] - b1);
-            l0 += x[0] + x[2];
-            l1 += x[1] + x[3];
-            const float w = sv[h] * unit;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] *= w;
+            const float* x = s[h];
             const __half2 h0 = __floats2half2_rn(x[0], x[1]), h1 = __floats2half2_rn(x[2], x[3]);
             p0[h] = transpose8(h2_bits(h0));
             p1[h] = transpose8(h2_bits(h1));
             if constexpr (SPLIT) {
                 const float2 y = __half22float2(h0), z = __half22float2(h1);
-                e0[h] = transpose8(h2_bits(__floats2half2_rn(x[0] - y.x, x[1] - y.y)));
-                e1[h] = transpose8(h2_bits(__floats2half2_rn(x[2] - z.x, x[3] - z.y)));
+                r0[h] = transpose8(h2_bits(__floats2half2_rn((x[0] - y.x) * kSecond, (x[1] - y.y) * kSecond)));
+                r1[h] = transpose8(h2_bits(__floats2half2_rn((x[2] - z.x) * kSecond, (x[3] - z.y) * kSecond)));
             }
         }
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                float sum[4];
+                float sum[4], rest[4];
 #pragma unroll
                 for (int h = 0; h < kPair; ++h) {
                     // Bytes 2b and 2b + 1 of two tokens, interleaved by value of d.
@@ -397,14 +439,21 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
                     const uint32_t a0 = bytes_to_h2(x, 0x4140), a1 = bytes_to_h2(x, 0x4342);
                     const uint32_t a2 = bytes_to_h2(y, 0x4140), a3 = bytes_to_h2(y, 0x4342);
                     if constexpr (SPLIT) {   // a pair's sum apart, added to the running one with rounding
-                        if (h == 0) mma_f16_first(sum, a0, a1, a2, a3, e0[h], e1[h]);
-                        else mma_f16(sum, a0, a1, a2, a3, e0[h], e1[h]);
-                        mma_f16(sum, a0, a1, a2, a3, p0[h], p1[h]);
+                        if (h == 0) {
+                            mma_f16_first(rest, a0, a1, a2, a3, r0[h], r1[h]);
+                            mma_f16_first(sum, a0, a1, a2, a3, p0[h], p1[h]);
+                        } else {
+                            mma_f16(rest, a0, a1, a2, a3, r0[h], r1[h]);
+                            mma_f16(sum, a0, a1, a2, a3, p0[h], p1[h]);
+                        }
                     } else {
                         mma_f16(o[2 * i + b], a0, a1, a2, a3, p0[h], p1[h]);
                     }
                 }
-                if constexpr (SPLIT) add4(o[2 * i + b], sum);
+                if constexpr (SPLIT) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) o[2 * i + b][x] += fmaf(rest[x], 1.f / kSecond, sum[x]);
+                }
             }
     }
 
@@ -427,12 +476,12 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
         sm_m[warp][2 * c] = m0; sm_m[warp][2 * c + 1] = m1;
         sm_l[warp][2 * c] = l0; sm_l[warp][2 * c + 1] = l1;
     }
-    const float back = ref > 0.f ? ref / kWeightScale : 1.f;
+    const float back0 = power(e0 - 7), back1 = power(e1 - 7);
 #pragma unroll
     for (int j = 0; j < KS; ++j) {
         const int x = r * (DP / 8) + 2 * j;
-        *reinterpret_cast<float2*>(&sm_o[warp][2 * c][x]) = make_float2(o[j][0] * back, o[j][2] * back);
-        *reinterpret_cast<float2*>(&sm_o[warp][2 * c + 1][x]) = make_float2(o[j][1] * back, o[j][3] * back);
+        *reinterpret_cast<float2*>(&sm_o[warp][2 * c][x]) = make_float2(o[j][0] * back0, o[j][2] * back0);
+        *reinterpret_cast<float2*>(&sm_o[warp][2 * c + 1][x]) = make_float2(o[j][1] * back1, o[j][3] * back1);
     }
     __syncthreads();
     auto factor = [](float m, float most) { return m == -INFINITY ? 0.f : exp2_hw(m - most); };

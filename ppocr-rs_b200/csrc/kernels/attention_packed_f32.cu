@@ -54,9 +54,6 @@ __device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-__device__ __forceinline__ float power(int e) { return __int_as_float((127 + e) << 23); }   // 2^e, -126 <= e <= 127
-__device__ __forceinline__ int exponent(float x) { return (__float_as_int(x) >> 23) - 127; }   // of x >= 0
-
 // a and b as FP16 pairs: the values rounded, and what is left.
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(a, b);

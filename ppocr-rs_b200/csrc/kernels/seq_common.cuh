@@ -121,6 +121,9 @@ struct Pack {
     }
 };
 
+__device__ __forceinline__ float power(int e) { return __int_as_float((127 + e) << 23); }   // 2^e, -126 <= e <= 127
+__device__ __forceinline__ int exponent(float x) { return (__float_as_int(x) >> 23) - 127; }   // of x >= 0
+
 // 2^x by the hardware unit (relative error about 2^-22; 0 for -infinity).
 __device__ __forceinline__ float exp2_hw(float x) {
     float y;

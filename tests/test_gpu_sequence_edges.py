@@ -251,3 +251,38 @@ def test_cached_small_value_scales(gpu, small, d, dtype):
     q = torch.randn(4, 4, d, device="cuda", generator=g).to(DT[dtype])
     out = cached(gpu, cache, q, lengths, table)
     check_cached_relative(out, q, cache, table, lengths, page, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("where", ["first", "middle", "last"])
+@pytest.mark.parametrize("power", [8, 12, 20, 27, 40, 60, 90])
+def test_cached_large_values_of_little_weight(gpu, power, where, dtype):
+    """A page whose values are 2^power times the others' but whose keys score far below: next to nothing."""
+    d, page, lengths = 64, 16, [333, 90, 5000]
+    g = ops.rng(power)
+    cache, table = ops.make_cache(g, lengths, 2, d, page)
+    cache.k.clamp_(-30, 30)
+    q = (0.5 + torch.rand(3, 4, d, device="cuda", generator=g)).to(DT[dtype])
+    for i, n in enumerate(lengths):
+        blocks = -(-n // page)
+        at = table[i, {"first": 0, "middle": blocks // 2, "last": blocks - 1}[where]].long()
+        cache.k[at] = -100
+        cache.k_scales[at] = (power * math.log(2) + 40) * 8 / (100 * 0.5 * d)   # scores of -40 - power ln 2 and less
+        cache.v_scales[at] = cache.v_scales[at] * 2.0 ** power
+    out = cached(gpu, cache, q, lengths, table)
+    check_cached_relative(out, q, cache, table, lengths, page, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_cached_value_scales_up_to_the_largest(gpu, dtype):
+    """Values near FP32's largest: those of ordinary pages next to them vanish, nothing overflows."""
+    d, page, lengths = 64, 16, [200, 40]
+    g = ops.rng(50)
+    cache, table = ops.make_cache(g, lengths, 2, d, page)
+    cache.k.clamp_(-3, 3)
+    cache.v.clamp_(-100, 100)
+    for i in range(2):
+        cache.v_scales[table[i, 1:3].long()] = 3e36
+    q = torch.randn(2, 4, d, device="cuda", generator=g).to(DT[dtype])
+    out = cached(gpu, cache, q, lengths, table)
+    check_cached_relative(out, q, cache, table, lengths, page, dtype)
