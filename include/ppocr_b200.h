@@ -588,6 +588,8 @@ int ppocr_gpu_synchronize(ppocr_gpu* gpu, void* stream, int timeout_ms);
  *   out = softmax(scale q k^T) v over the sequence's keys; causal: query j of
  *   a sequence of nq queries and nk keys sees keys 0 .. j + nk - nq.
  * A query that sees no key, or whose scores are all -infinity, gives zeros.
+ * FP32 values of q, k and v count to 2^-22 of themselves, but no finer than 2^-50
+ * of the largest of their token and head.
  * Masked keys and values never reach an output, whatever they hold.  Tokens of
  * `out` outside every sequence are left as they were.  d: 1..128; heads a
  * multiple of kv_heads; scale: 0 (d^-1/2) or positive, up to 1e30.  The recognizers' encoder

@@ -5,9 +5,13 @@
 // power of two, and a product as its three leading ones: FP32-class, at half
 // the tensor-core time of TF32 pieces (whose MMAs hold half the values).  FP16's
 // range is met by one power of two per row of Q, K and V, the one that takes the
-// row's largest magnitude into [2^8, 2^9): Q's and K's multiply the scores, and
+// row's largest magnitude into [2^14, 2^15): Q's and K's multiply the scores, and
 // V's the weights before these are split in turn.  A row's own power, and not a
 // tile's, so that a key which a query must not see cannot touch its precision.
+// Second pieces are held times 2^11 and their products summed apart: so FP16's
+// least step cuts a value at 2^-50 of its row's largest, and one down to 2^-28 of
+// it, a channel next to a far larger one, has its 22 bits.  (With both pieces in
+// the same power that ended at 2^-16, and 2^-30 kept four bits.)
 //
 // A block owns 64 rows of one (sequence, KV head): the `group` query heads
 // that share the KV head are rows too, so K and V are read once per group.
@@ -26,9 +30,9 @@
 // Chunks of 3 requests, 16 heads of 64, 4 KV heads: 78 us (TF32 pieces split by
 // each warp: 165).  64 lines of 4 to 200 tokens, 8 heads of 15: 27 us, latency.
 //
-// Softmax: weights are relative to a maximum that moves only when a score passes
-// it by more than 4 (in log2), so most tiles need no reduction; likewise the
-// power of two that weight x V's power is taken relative to.
+// Softmax: weights are relative to the maximum + 4 (in log2) when it last moved,
+// and it moves when a score passes that, so most tiles need no reduction; likewise
+// the power of two that weight x V's power is taken relative to.
 #include <cuda_fp16.h>
 
 #include "attention_packed.cuh"
@@ -38,7 +42,7 @@ namespace ppocr {
 namespace {
 
 constexpr int kKeys = 32, kPad = 8;
-constexpr float kSlack = 4.f;
+constexpr float kSlack = 4.f;   // log2 of what weights leave above the maximum: at most 1, they may meet any V row's power
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -54,11 +58,13 @@ __device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-// a and b as FP16 pairs: the values rounded, and what is left.
+// a and b as FP16 pairs: the values rounded, and what is left times 2^11 (no more
+// than the value, so it is never out of range, and 2^-11 of FP16's least step counts).
+constexpr float kSecond = 2048.f;
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(a, b);
     const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    const __half2 l = __floats2half2_rn((a - f.x) * kSecond, (b - f.y) * kSecond);
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
@@ -97,7 +103,7 @@ struct Rows {
         }
     }
     // The rows' planes, and done(n, top, e) by one thread for row n, which holds
-    // its values times 2^(8 - e); top is its largest magnitude.
+    // its values times 2^(14 - e); top is its largest magnitude.
     template <typename Done>
     static __device__ __forceinline__ void split(const float4* raw, __half* hi, __half* lo, Done done) {
         const int tid = threadIdx.x;
@@ -112,8 +118,8 @@ struct Rows {
             }
 #pragma unroll
             for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const int e = min(max(exponent(top), -100), 120), n = tid / kLanes + kPerPass * i;
-            const float up = power(8 - e);
+            const int e = min(max(exponent(top), -100), 127), n = tid / kLanes + kPerPass * i;
+            const float up = power(14 - e);
 #pragma unroll
             for (int j = 0; j < kPieces; ++j) {
                 uint2 h, l;
@@ -130,7 +136,7 @@ struct Rows {
 
 // What a row of Q or K was divided by.  Rows of 2^60 and more are left to
 // attend_row: the factors' product might overflow where the score does not.
-__device__ __forceinline__ float score_factor(float top, int e) { return top < power(60) ? power(e - 8) : NAN; }
+__device__ __forceinline__ float score_factor(float top, int e) { return top < power(60) ? power(e - 14) : NAN; }
 
 // What a block of WARPS warps, 16 rows each, keeps in shared memory.  With two
 // buffers of planes the next tile is split while this one is worked on.
@@ -205,7 +211,7 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS)
 #pragma unroll
         for (int x = 0; x < 4; ++x) o[i][x] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, b0 = 0.f, b1 = 0.f, l0 = 0.f, l1 = 0.f;   // b: m, 0 while it is -infinity
-    int e0 = -100, e1 = -100;            // o holds sums of weight x V, times 2^(16 - e)
+    int e0 = -100, e1 = -100;            // o holds sums of weight x V, times 2^(22 - e)
     float unit0 = power(108), unit1 = power(108);   // 2^(8 - e)
 
     if (tiles > 0) {
@@ -259,8 +265,8 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS)
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     const float fx = x ? f.y : f.x;
-                    s[n][x] = (s[n][x] + rest[n][x]) * (f0 * fx);
-                    s[n][x + 2] = (s[n][x + 2] + rest[n][x + 2]) * (f1 * fx);
+                    s[n][x] = fmaf(rest[n][x], 1.f / kSecond, s[n][x]) * (f0 * fx);
+                    s[n][x + 2] = fmaf(rest[n][x + 2], 1.f / kSecond, s[n][x + 2]) * (f1 * fx);
                 }
             }
             if ((j + 1) * kKeys > sure) {
@@ -278,11 +284,12 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS)
                 t0 = fmaxf(t0, fmaxf(s[n][0], s[n][1]));
                 t1 = fmaxf(t1, fmaxf(s[n][2], s[n][3]));
             }
-            if (__any_sync(0xffffffffu, t0 > m0 + kSlack || t1 > m1 + kSlack)) {
+            if (__any_sync(0xffffffffu, t0 > m0 || t1 > m1)) {
                 auto raise = [&](float t, float& m, float& b, float& l, int& e, float& unit, int half) {
                     t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-                    t = fmaxf(m, fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2)));
-                    if (t > m + kSlack) {   // the whole row's four lanes; a row's steps depend on its own scores alone
+                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+                    if (t > m) {   // the whole row's four lanes; a row's steps depend on its own scores alone
+                        t += kSlack;
                         // What the sums hold shrinks with the weights, so their power may fall as far.
                         const float fall = m - t;   // -infinity for the first keys
                         const int next = max(e + (int)fmaxf(ceilf(fall), -300.f), -100);
@@ -354,18 +361,18 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS)
                 }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    float sum[4];   // the small products first
-                    mma_first(sum, wl[0], bh[0][2 * u], bh[0][2 * u + 1]);
-                    mma(sum, wh[0], bl[0][2 * u], bl[0][2 * u + 1]);
+                    float sum[4], small[4];
+                    mma_first(small, wl[0], bh[0][2 * u], bh[0][2 * u + 1]);
+                    mma_first(sum, wh[0], bh[0][2 * u], bh[0][2 * u + 1]);
+                    mma(small, wh[0], bl[0][2 * u], bl[0][2 * u + 1]);
 #pragma unroll
                     for (int n = 1; n < NT / 2; ++n) {
-                        mma(sum, wl[n], bh[n][2 * u], bh[n][2 * u + 1]);
-                        mma(sum, wh[n], bl[n][2 * u], bl[n][2 * u + 1]);
+                        mma(small, wl[n], bh[n][2 * u], bh[n][2 * u + 1]);
+                        mma(sum, wh[n], bh[n][2 * u], bh[n][2 * u + 1]);
+                        mma(small, wh[n], bl[n][2 * u], bl[n][2 * u + 1]);
                     }
 #pragma unroll
-                    for (int n = 0; n < NT / 2; ++n) mma(sum, wh[n], bh[n][2 * u], bh[n][2 * u + 1]);
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) o[i + u][x] += sum[x];
+                    for (int x = 0; x < 4; ++x) o[i + u][x] += fmaf(small[x], 1.f / kSecond, sum[x]);
                 }
             }
         }
@@ -382,7 +389,7 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS)
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
     const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
-    const float u0 = power(e0 - 16), u1 = power(e1 - 16);
+    const float u0 = power(e0 - 22), u1 = power(e1 - 22);
     float* out = at.template queries<float>(p.out);
     bool bad[2] = {false, false};
 #pragma unroll

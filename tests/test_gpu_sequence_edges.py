@@ -286,3 +286,40 @@ def test_cached_value_scales_up_to_the_largest(gpu, dtype):
     q = torch.randn(2, 4, d, device="cuda", generator=g).to(DT[dtype])
     out = cached(gpu, cache, q, lengths, table)
     check_cached_relative(out, q, cache, table, lengths, page, dtype)
+
+
+# ---------------------------------------------------------------------------
+# FP32: channels far apart
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n", [40, 300])
+@pytest.mark.parametrize("d", [15, 64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("apart", [16, 22, 28])
+def test_packed_fp32_channels_of_different_powers(gpu, n, d, causal, apart):
+    """Columns of V up to 2^-apart of the others keep FP32's precision, and so do the products of a small channel of
+    q with a large one of k."""
+    g = ops.rng(n + apart)
+    q, k, v = (torch.randn(n, h, d, device="cuda", generator=g) for h in (4, 2, 2))
+    down = torch.exp2(-torch.randint(0, apart + 1, (d,), device="cuda", generator=g).float())
+    v *= down
+    other = torch.exp2(-torch.randint(0, apart + 1, (d,), device="cuda", generator=g).float())
+    q, k = q * other, k / other
+    out = packed(gpu, q, k, v, [n], [n], causal)
+    ref, tol = ops.packed_reference(q, k, v, [n], [n], causal, d ** -0.5, "f32")
+    ops.check(out, ref, tol)
+
+
+@pytest.mark.parametrize("n", [40, 300])
+@pytest.mark.parametrize("apart", [40, 70])
+def test_packed_fp32_channels_too_far_apart(gpu, n, apart):
+    """Beyond that a value keeps 2^-50 of its row's largest, twice over two roundings of it and its weight."""
+    d = 64
+    g = ops.rng(n + apart)
+    q, k, v = (torch.randn(n, 2, d, device="cuda", generator=g) for _ in range(3))
+    v[..., ::3] *= 2.0 ** -apart
+    out = packed(gpu, q, k, v, [n], [n])
+    ref, mag, prod = ops.attend(q.double(), k.double(), v.double(), d ** -0.5)
+    row = v.abs().amax(-1, keepdim=True).expand(-1, -1, d).double()
+    most = ops.attend(q.double(), k.double(), row, d ** -0.5)[0]
+    ops.check(out, ref, ops.tolerance(ref, mag, prod, d, n, "f32", 2.0 ** -20) + most * 2.0 ** -49)
