@@ -18,14 +18,15 @@
 // when a product would pass FP16's range, down with the weights when the maximum
 // moves.  So pages of large values and no weight cost the others no bits.  (A
 // power of the V scales alone does: at 2^27 between two pages the weights of the
-// smaller one had three bits left.)  The weights' second piece is held times
-// 2^11 and summed apart, which keeps 22 bits down to 2^-20 of the largest product.
+// smaller one had three bits left.)  Second pieces are held times 2^11
+// and their products summed apart, which keeps 22 bits of weights down to 2^-20 of
+// the largest product and of q's values down to 2^-28 of the head's largest.
 //
 // A warp owns every fourth pair of tiles of its block's token range, fetches
 // them with cp.async into a ring of its own in shared memory (two pairs; no
-// barrier of the block is involved) and keeps its own softmax state; the running
-// maximum moves only when a score passes it by more than 8 (weights up to 2^8),
-// so most tiles need no reduction at all.  The two tiles of a pair are two
+// barrier of the block is involved) and keeps its own softmax state; weights are
+// relative to the maximum + 6 (in log2) when it last moved, and it moves when a
+// score passes that, so most tiles need no reduction at all.  The two tiles of a pair are two
 // independent chains of products.  The range of a sequence is split over the
 // blocks of a cluster (1 to 16) when there are few sequences and heads; warps
 // join through shared memory, blocks through distributed shared memory, both in
@@ -250,10 +251,10 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // Power of two that takes the head's largest value into [2^8, 2^9).
-        const int e = max((int)(__float_as_uint(top) >> 23) - 127, -100);
-        const float up = __uint_as_float((uint32_t)(127 + 8 - e) << 23);
-        qscale = p.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - 8 + e) << 23);
+        // Power of two that takes the head's largest value into [2^14, 2^15).
+        const int e = max(exponent(top), -100);
+        const float up = power(14 - e);
+        qscale = p.scale * 1.4426950408889634f * power(e - 14);
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
                 qh[s][h] = h2_bits(hi);
                 if constexpr (SPLIT) {
                     const float2 f = __half22float2(hi);
-                    ql[s][h] = h2_bits(__floats2half2_rn(isinf(f.x) ? 0.f : a - f.x, isinf(f.y) ? 0.f : b - f.y));
+                    ql[s][h] = h2_bits(__floats2half2_rn(isinf(f.x) ? 0.f : (a - f.x) * kSecond, isinf(f.y) ? 0.f : (b - f.y) * kSecond));
                 }
             }
     }
@@ -324,7 +325,10 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
                     mma_f16(s[h], a0, a1, a2, a3, qh[i][0], qh[i][1]);
                 }
             }
-            if constexpr (SPLIT) add4(s[h], rest);
+            if constexpr (SPLIT) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[h][i] = fmaf(rest[i], 1.f / kSecond, s[h][i]);
+            }
             const float k0 = f0 * sk, k1 = f1 * sk;
             s[h][0] *= k0; s[h][1] *= k1;
             s[h][2] *= k0; s[h][3] *= k1;

@@ -323,3 +323,18 @@ def test_packed_fp32_channels_too_far_apart(gpu, n, apart):
     row = v.abs().amax(-1, keepdim=True).expand(-1, -1, d).double()
     most = ops.attend(q.double(), k.double(), row, d ** -0.5)[0]
     ops.check(out, ref, ops.tolerance(ref, mag, prod, d, n, "f32", 2.0 ** -20) + most * 2.0 ** -49)
+
+
+@pytest.mark.parametrize("d", [24, 64, 128])
+@pytest.mark.parametrize("apart", [16, 22, 28])
+def test_cached_fp32_query_channels_of_different_powers(gpu, d, apart):
+    """The small channels of a query count where the large ones meet keys of 0."""
+    g = ops.rng(apart + d)
+    lengths, page = [40, 1000], 16
+    cache, table = ops.make_cache(g, lengths, 2, d, page)
+    q = torch.randn(2, 4, d, device="cuda", generator=g)
+    cache.k[..., :4] = 0
+    q[..., 4:] *= 2.0 ** -apart
+    cache.k_scales *= 2.0 ** apart
+    out = cached(gpu, cache, q, lengths, table)
+    check_cached_relative(out, q, cache, table, lengths, page, "f32")
