@@ -238,6 +238,9 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
     // B operand of the scores: head r's values of d, in the order in which the
     // lane's K bytes come; b0 holds bytes 4s, 4s + 1 and b1 bytes 4s + 2, 4s + 3.
     uint32_t qh[KS][2], ql[SPLIT ? KS : 1][2];
+    // Scores are divided by a head's power, times its K scale and the call's: a scale
+    // above 1 last, since its product with the power may overflow where the score does not.
+    const float scale = p.scale * 1.4426950408889634f, first = fminf(scale, 1.f), last = fmaxf(scale, 1.f);
     float qscale;
     {
         float x[DP / 4];
@@ -254,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
         // Power of two that takes the head's largest value into [2^14, 2^15).
         const int e = max(exponent(top), -100);
         const float up = power(14 - e);
-        qscale = p.scale * 1.4426950408889634f * power(e - 14);
+        qscale = first * power(e - 14);
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -329,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[h][i] = fmaf(rest[i], 1.f / kSecond, s[h][i]);
             }
-            const float k0 = f0 * sk, k1 = f1 * sk;
+            const float k0 = f0 * sk * last, k1 = f1 * sk * last;
             s[h][0] *= k0; s[h][1] *= k1;
             s[h][2] *= k0; s[h][3] *= k1;
             // Past the sequence's end, or on a page that is none.

@@ -338,3 +338,49 @@ def test_cached_fp32_query_channels_of_different_powers(gpu, d, apart):
     cache.k_scales *= 2.0 ** apart
     out = cached(gpu, cache, q, lengths, table)
     check_cached_relative(out, q, cache, table, lengths, page, "f32")
+
+
+# ---------------------------------------------------------------------------
+# Scales and queries whose product passes FP32 while the scores do not
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [40, 700])
+@pytest.mark.parametrize("d", [16, 64])
+def test_packed_negative_scores_of_large_scales(gpu, n, d, dtype):
+    """Every score finite and negative: the least negative one's value."""
+    g = ops.rng(n)
+    q, k = torch.zeros(n, 1, d, device="cuda"), torch.zeros(n, 1, d, device="cuda")
+    q[..., 1] = 2.0 ** 45
+    k[..., 1] = -(1 + torch.rand(n, 1, device="cuda", generator=g)) * 2.0 ** -20
+    k[n // 2, 0, 1] = -2.0 ** -21
+    v = torch.randn(n, 1, d, device="cuda", generator=g)
+    q, k, v = (x.to(DT[dtype]) for x in (q, k, v))
+    out = packed(gpu, q, k, v, [n], [n], scale=1e30)
+    ref = v[n // 2].double().expand(n, 1, d)
+    ops.check(out, ref, ref.abs() * (2 * HALF_STEP[dtype] + 2.0 ** -20) + 1e-30)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("power,scale", [(45, 1e30), (90, 1.0), (60, 1e-20)])
+def test_cached_negative_scores_of_large_scales(gpu, power, scale, dtype):
+    g = ops.rng(power)
+    lengths, page, d = [90, 1000], 16, 64
+    cache, table = ops.make_cache(g, lengths, 1, d, page)
+    cache.k.zero_()
+    cache.k[..., 2] = torch.randint(-128, -100, cache.k.shape[:3], device="cuda", generator=g).to(torch.int8)
+    cache.k_scales.fill_(2.0 ** (100 - power) / scale)   # scores near -2^107
+    at = [(0, 47), (1, 733)]
+    for i, t in at:
+        cache.k[table[i, t // page].long(), 0, t % page, 2] = -50
+    q = torch.zeros(2, 3, d, device="cuda")
+    q[..., 2] = 2.0 ** power
+    q = q.to(DT[dtype])
+    s = torch.cuda.current_stream()
+    out = torch.full_like(q, 7.0)
+    gpu.attention_cached(cache, q, torch.tensor(lengths, dtype=torch.int32, device="cuda"), table, out, scale=scale, stream=s)
+    gpu.synchronize(s)
+    for i, t in at:
+        row = table[i, t // page].long()
+        ref = (cache.v[row, 0, t % page].double() * cache.v_scales[row, 0].double()).expand(3, d)
+        ops.check(out[i], ref, ref.abs() * (HALF_STEP[dtype] + (2.0 ** -11 if dtype == "bf16" else 2.0 ** -20)) + 1e-30)
