@@ -578,7 +578,10 @@ typedef struct ppocr_tokens {
 /* Waits (bounded by timeout_ms; <= 0: 60 s) for `stream` (NULL: the handle's
  * own), then raises and clears what the sequence operators reported since the
  * last call: PPOCR_ERR_INVALID_INPUT for a bad offset, length, table entry, id
- * or state, PPOCR_ERR_GPU for a tensor-core pipeline wait that ran out. */
+ * or state, PPOCR_ERR_GPU for a tensor-core pipeline wait that ran out.  A
+ * report is the handle's, whichever stream it came from, and is raised once: the
+ * results of every stream with calls since the last synchronize are then in
+ * doubt.  A program that wants its streams' reports apart uses a handle each. */
 int ppocr_gpu_synchronize(ppocr_gpu* gpu, void* stream, int timeout_ms);
 
 /* Attention over packed sequences: sequence i's queries are the tokens

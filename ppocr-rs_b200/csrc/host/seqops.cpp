@@ -11,6 +11,7 @@
 
 #include "../kernels/seq.h"
 #include "handles.hpp"
+#include "seq_status.hpp"
 
 using namespace ppocr;
 
@@ -141,9 +142,7 @@ int ppocr_gpu_synchronize(ppocr_gpu* gpu, void* stream, int timeout_ms) {
         if (!gpu) fail(PPOCR_ERR_INVALID_INPUT, "gpu handle is null");
         OnDevice on(gpu);
         wait_stream(stream_of(gpu, stream), timeout_ms, gpu);
-        volatile int* status = gpu->seq_status;
-        const int bad = status[0], wait = status[1];
-        status[0] = status[1] = 0;
+        const int bad = take_status(gpu->seq_status), wait = take_status(gpu->seq_status + 1);
         if (wait)
             fail(PPOCR_ERR_GPU, "GPU error: a tensor-core pipeline wait ran out (code " + std::to_string(wait) +
                                     "); the results are incomplete");
