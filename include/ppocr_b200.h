@@ -581,7 +581,10 @@ typedef struct ppocr_tokens {
  * or state, PPOCR_ERR_GPU for a tensor-core pipeline wait that ran out.  A
  * report is the handle's, whichever stream it came from, and is raised once: the
  * results of every stream with calls since the last synchronize are then in
- * doubt.  A program that wants its streams' reports apart uses a handle each. */
+ * doubt.  A program that wants its streams' reports apart uses a handle each.
+ * When the time runs out the call fails with PPOCR_ERR_GPU; nothing is cleared,
+ * and after a wait for the handle's own stream, as in a forward, the handle
+ * accepts no further work. */
 int ppocr_gpu_synchronize(ppocr_gpu* gpu, void* stream, int timeout_ms);
 
 /* Attention over packed sequences: sequence i's queries are the tokens

@@ -141,7 +141,9 @@ int ppocr_gpu_synchronize(ppocr_gpu* gpu, void* stream, int timeout_ms) {
     return guard([&] {
         if (!gpu) fail(PPOCR_ERR_INVALID_INPUT, "gpu handle is null");
         OnDevice on(gpu);
-        wait_stream(stream_of(gpu, stream), timeout_ms, gpu);
+        // The caller's stream may hold work of its own that takes longer than it cares to
+        // wait here: only the handle's own stream condemns the handle.
+        wait_stream(stream_of(gpu, stream), timeout_ms, stream ? nullptr : gpu);
         const int bad = take_status(gpu->seq_status), wait = take_status(gpu->seq_status + 1);
         if (wait)
             fail(PPOCR_ERR_GPU, "GPU error: a tensor-core pipeline wait ran out (code " + std::to_string(wait) +

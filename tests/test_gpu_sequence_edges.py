@@ -384,3 +384,27 @@ def test_cached_negative_scores_of_large_scales(gpu, power, scale, dtype):
         row = table[i, t // page].long()
         ref = (cache.v[row, 0, t % page].double() * cache.v_scales[row, 0].double()).expand(3, d)
         ops.check(out[i], ref, ref.abs() * (HALF_STEP[dtype] + (2.0 ** -11 if dtype == "bf16" else 2.0 ** -20)) + 1e-30)
+
+
+# ---------------------------------------------------------------------------
+# Waiting
+# ---------------------------------------------------------------------------
+
+def test_waiting_for_a_busy_stream_of_the_callers_leaves_the_handle_usable():
+    gpu = P.Gpu(0)
+    s = torch.cuda.Stream()
+    x = torch.randn(2, 100, device="cuda")
+    bad = torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+    mask = torch.full((2, 4), -1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    gpu.logit_rules(x, torch.empty_like(x), mask=mask, mask_index=bad, stream=s)
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(400_000_000)   # about 0.2 s
+    with pytest.raises(P.GpuError, match="wait limit"):
+        gpu.synchronize(s, timeout_ms=5)
+    with pytest.raises(P.InvalidInput, match="out of range"):   # still to be reported
+        gpu.synchronize(s)
+    out = gpu.logit_rules(x, torch.empty_like(x), bias=torch.ones(100, device="cuda"), stream=s)
+    gpu.synchronize(s)
+    assert torch.equal(out, x + 1)
+    gpu.close()
