@@ -427,8 +427,8 @@ def _cuda_stream(stream):
 def _attention_scale(scale) -> float:
     if scale is None:
         return 0.0   # the library's default, d^-1/2
-    if not scale > 0:
-        raise InvalidInput("invalid input: scale must be positive")
+    if not scale > 2.0 ** -150:   # what rounds to 0 in FP32 would mean the default
+        raise InvalidInput("invalid input: scale must be positive, in FP32 too")
     return scale
 
 
