@@ -408,3 +408,82 @@ def test_waiting_for_a_busy_stream_of_the_callers_leaves_the_handle_usable():
     gpu.synchronize(s)
     assert torch.equal(out, x + 1)
     gpu.close()
+
+
+# ---------------------------------------------------------------------------
+# Offsets past 32 bits, the smallest scales
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_pages_past_32_bits(gpu, dtype):
+    """Pages 2^31 and 2^32 bytes into the cache answer as the same ones of a small cache do."""
+    page, kv, d, lengths = 128, 8, 128, [700, 129]
+    cell = page * kv * d
+    pages = 2 ** 32 // cell + 9
+    g = ops.rng(60)
+    small, table = ops.make_cache(g, lengths, kv, d, page)
+    n = small.k.shape[0]
+    places = torch.tensor([0, 2 ** 31 // cell - 1, 2 ** 31 // cell, 2 ** 32 // cell - 1, 2 ** 32 // cell, pages - 1] +
+                          list(range(7, 7 + n)), device="cuda")[:n]
+    big = P.PagedCache(*(torch.empty(pages, *x.shape[1:], dtype=x.dtype, device="cuda")
+                         for x in (small.k, small.v, small.k_scales, small.v_scales)))
+    for x, y in zip((big.k, big.v, big.k_scales, big.v_scales), (small.k, small.v, small.k_scales, small.v_scales)):
+        x[places] = y
+    far = torch.where(table >= 0, places[table.clamp_min(0).long()].int(), -1)
+    s = torch.cuda.current_stream()
+    held = torch.tensor([690, 120], dtype=torch.int32, device="cuda")
+    new = [torch.randn(19, kv, d, device="cuda", generator=g).to(DT[dtype]) for _ in range(2)]
+    q = torch.randn(2, 16, d, device="cuda", generator=g).to(DT[dtype])
+    outs = []
+    for cache, where in ((small, table), (big, far)):
+        gpu.cache_append(cache, *new, ops.offsets([10, 9]), held, where, stream=s)
+        k, v = (torch.empty(sum(lengths), kv, d, dtype=DT[dtype], device="cuda") for _ in range(2))
+        gpu.cache_read(cache, k, v, ops.offsets(lengths), torch.zeros_like(held), where, stream=s)
+        outs.append([k, v, cached(gpu, cache, q, lengths, where)])
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [5, 9])
+@pytest.mark.parametrize("d", [15, 64])
+def test_packed_strides_past_32_bits(gpu, n, d, dtype):
+    """Tokens 2^29 and more values apart."""
+    step = 2 ** 29 + 64
+    g = ops.rng(n)
+    whole = torch.empty((n - 1) * step + 3 * d, dtype=DT[dtype], device="cuda")
+    q, k, v = (whole[i * d:].as_strided((n, 1, d), (step, d, 1)) for i in range(3))
+    near = [torch.randn(n, 1, d, device="cuda", generator=g).to(DT[dtype]) for _ in range(3)]
+    for x, y in zip((q, k, v), near):
+        x.copy_(y)
+    out = packed(gpu, *near, [n], [n], True)
+    far = torch.empty_like(near[0])
+    s = torch.cuda.current_stream()
+    gpu.attention_packed(q, k, v, ops.offsets([n]), ops.offsets([n]), far, causal=True, stream=s)
+    gpu.synchronize(s)
+    assert torch.equal(out, far)
+    gpu.attention_packed(*near, ops.offsets([n]), ops.offsets([n]), q, causal=True, stream=s)
+    gpu.synchronize(s)
+    assert torch.equal(out, q) and torch.equal(k, near[1]) and torch.equal(v, near[2])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [40, 700])
+def test_the_smallest_scales_weigh_all_keys_alike(gpu, n, dtype):
+    g = ops.rng(n)
+    d, page = 64, 16
+    q, k, v = (torch.randn(n, 2, d, device="cuda", generator=g).to(DT[dtype]) for _ in range(3))
+    weight = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -20
+    for scale in (2.0 ** -149, 1e-38):
+        out = packed(gpu, q, k, v, [n], [n], True, scale=scale)
+        zero = torch.zeros_like(q).double()
+        ref, mag, prod = ops.attend(zero, zero, v.double(), 1.0, 0)
+        ops.check(out, ref, ops.tolerance(ref, mag, prod, d, n, dtype, weight))
+        cache, table = ops.make_cache(g, [n], 2, d, page)
+        s = torch.cuda.current_stream()
+        one = torch.empty_like(q[:1])
+        gpu.attention_cached(cache, q[:1], torch.tensor([n], dtype=torch.int32, device="cuda"), table, one, scale=scale, stream=s)
+        gpu.synchronize(s)
+        kk, vv = ops.cache_values(cache, table, 0, n, page)
+        ref, mag, prod = ops.attend(zero[:1], torch.zeros_like(kk), vv, 1.0)
+        ops.check(one, ref, ops.tolerance(ref, mag, prod, d, n, dtype, 2.0 ** -11 if dtype == "bf16" else 2.0 ** -20))
