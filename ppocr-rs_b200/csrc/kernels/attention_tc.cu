@@ -324,6 +324,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                 // The stage, and tile 0's first weights.
                 const bool own = lane && j < n[0];
                 wait(own ? &p_full[0][0] : &full[s], own ? j & 1 : phase, 3);
+                if (ok && (j + 1) * kKeys > w.ks.len) {
+                    // The last tile's rows of V behind the sequence belong to others, and a
+                    // weight of 0 times an infinity or NaN there would send every row of the
+                    // CTA to the second computation (2,000 tokens with NaN behind them: 84 ms
+                    // instead of 0.06).
+                    __syncwarp();
+                    for (int c = 0; c < DC; ++c)
+                        for (int at = (w.ks.len - j * kKeys) * 128 + lane * 16; at < kChunk; at += 512)
+                            *reinterpret_cast<uint4*>(ring + s * L::stage_bytes + c * kChunk + at) = make_uint4(0, 0, 0, 0);
+                    tc::fence_proxy_async();
+                    __syncwarp();
+                }
                 const uint32_t v = v_desc + s * (L::stage_bytes >> 4), k = k_desc + s * (L::stage_bytes >> 4);
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t) {
