@@ -553,7 +553,8 @@ int ppocr_selftest_dispatch(size_t workers, size_t items, uint32_t stall_mask, u
  * key / value cache with its single-token attention, and logit rules, on
  * device memory that the caller owns.
  *
- * Every call enqueues one kernel (none for an empty input) on `stream` (a
+ * Every call enqueues one kernel (none for an empty input; logit rules with
+ * histories one for every 65,535 rows) on `stream` (a
  * cudaStream_t of the handle's device; NULL = the handle's own stream, as in
  * ppocr_model_run; the legacy default stream is passed as cudaStreamLegacy)
  * and returns.  They allocate nothing, use no workspace and keep no state in
@@ -566,7 +567,10 @@ int ppocr_selftest_dispatch(size_t workers, size_t items, uint32_t stall_mask, u
  * pointers are checked by the call (PPOCR_ERR_INVALID_INPUT).  Offsets,
  * lengths, block tables, ids and states live on the device, so the kernels
  * check them: a bad one is never followed out of bounds, what it stands for
- * is left out, and the next ppocr_gpu_synchronize reports it. */
+ * is left out (tokens that clamped offsets give to two sequences get either's
+ * result), and the next ppocr_gpu_synchronize reports it.  The 16 bytes that a
+ * handle's reports are written to are never given back, since a captured graph may
+ * outlive the handle. */
 enum ppocr_dtype { PPOCR_DTYPE_F32 = 0, PPOCR_DTYPE_BF16 = 1 };
 
 /* A device tensor [tokens][heads][d]. */
@@ -597,7 +601,11 @@ int ppocr_gpu_synchronize(ppocr_gpu* gpu, void* stream, int timeout_ms);
  * FP32 values of q, k and v count to 2^-22 of themselves, but no finer than 2^-50
  * of the largest of their token and head.
  * Masked keys and values never reach an output, whatever they hold.  Tokens of
- * `out` outside every sequence are left as they were.  d: 1..128; heads a
+ * `out` outside every sequence are left as they were.  Rows that come out
+ * non-finite, rows of scores beyond 2^24 (BF16) and of q or k beyond 2^60 (FP32)
+ * are computed a second time by one warp each: a call of 2,000 tokens, 16 heads of
+ * 128 that are all such rows takes 80 ms, and the time grows with the square of
+ * the length.  d: 1..128; heads a
  * multiple of kv_heads; scale: 0 (d^-1/2) or positive, up to 1e30.  The recognizers' encoder
  * attention (src/cpu/model.rs:1705-1725) is the case of equal lengths. */
 typedef struct ppocr_attention_packed_args {
@@ -634,7 +642,7 @@ typedef struct ppocr_block_table {
 
 /* Appends the tokens [offsets[i], offsets[i + 1]) of k and v to sequence i,
  * which holds held[i] tokens.  A page's scale per head is the largest
- * magnitude it has seen / 127: where new tokens raise the scale of a
+ * magnitude it has seen x (1 / 127), both in FP32: where new tokens raise the scale of a
  * part-filled page, the integers it holds are rounded again.  A page's first
  * token starts it afresh, whatever it held.  Integers are round(value / scale)
  * of the exact quotient, ties to even; a value that is not finite makes its
@@ -667,7 +675,9 @@ int ppocr_cache_read(ppocr_gpu* gpu, const ppocr_cache_read_args* args, void* st
 
 /* Single-token attention: one query per sequence over the first lengths[i]
  * tokens of its pages; a length of 0 gives zeros.  q and out are
- * [sequences][heads][d]; scale as in ppocr_attention_packed. */
+ * [sequences][heads][d]; scale as in ppocr_attention_packed.  A token's softmax
+ * weight x V scale counts to 2^-11 of itself (BF16 calls; 2^-22 in FP32 ones), but
+ * no finer than 2^-31 (2^-42) of the largest of its head. */
 typedef struct ppocr_attention_cached_args {
     int dtype;                   /* of q and out */
     int heads;

@@ -3,7 +3,7 @@
 // A page holds `page` consecutive tokens of one sequence for every head, as
 // integers in [-127, 127]; the values they stand for are integer x scale with
 // one FP32 scale per (page, head), the largest magnitude the page's head has
-// seen / 127.  Appending to a part-filled page whose scale grows rounds the
+// seen x FP32's 1 / 127.  Appending to a part-filled page whose scale grows rounds the
 // integers that it held again: q' = round(q s_before / s).  Every rounding to
 // an integer is that of the exact quotient (ties to even), so the cache's
 // contents depend on the values alone.
