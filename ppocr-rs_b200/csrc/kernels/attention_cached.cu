@@ -33,11 +33,11 @@
 // a fixed order: one launch, no workspace.  The longest sequences start first.
 //
 // Measured: 64 sequences of 1 to 4,100 tokens, 32 heads on 8 KV heads of 128, pages
-// of 32, BF16: 68 us (4.1 TB/s; 115 with the loads straight to registers, 75
-// without the order of sequences).  Two of up to 65,000 tokens, 24 heads, FP32: 92
-// us (2.6 TB/s).  One of 101 tokens: 4.5 us.  The instructions between the loads
+// of 32, BF16: 70 us (4.0 TB/s; 68 with weights relative to the V scales alone, then
+// 115 with the loads straight to registers, 75 without the order of sequences).  Two
+// of up to 65,000 tokens, 24 heads, FP32: 89 us (2.6 TB/s).  One of 101 tokens: 4.8 us.  The instructions between the loads
 // and the MMAs (a byte_perm and a subtraction per two values, and the softmax:
-// 456 per 16 tokens of d = 128) keep the issue slots 57 % busy while four of eight
+// 470 per 16 tokens of d = 128) keep the issue slots 56 % busy while four of eight
 // columns of N are live, and are what is left above the bytes.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>

@@ -17,7 +17,7 @@
 // (35 MB, 5.4 us at the copy rate): 45.7 us with six blocks per SM, 48.9 with
 // five, 57.9 with eight (registers spilled).  The issue slots are then 70 % busy, so
 // instructions count next: with the scale in the exponent's multiply-add, masks only
-// where a tile needs them and 32-bit divisions and strides, 41.6 us.
+// where a tile needs them and 32-bit divisions and strides, 41.8 us.
 #include "attention_packed.cuh"
 
 namespace ppocr {

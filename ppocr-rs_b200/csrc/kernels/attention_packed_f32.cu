@@ -27,8 +27,9 @@
 // Bound: the tensor cores (three products) together with splitting, 1 us of
 // every 4 where it stood between two barriers; with eight warps one half of
 // them splits the next tile while the other half multiplies (95 -> 89 us).
-// Chunks of 3 requests, 16 heads of 64, 4 KV heads: 78 us (TF32 pieces split by
-// each warp: 165).  64 lines of 4 to 200 tokens, 8 heads of 15: 27 us, latency.
+// Chunks of 3 requests, 16 heads of 64, 4 KV heads: 80 to 85 us (second pieces in
+// the first ones' power: 1 us less; TF32 pieces split by each warp: 165).  64 lines
+// of 4 to 200 tokens, 8 heads of 15: 28 us, latency.
 //
 // Softmax: weights are relative to the maximum + 4 (in log2) when it last moved,
 // and it moves when a score passes that, so most tiles need no reduction; likewise

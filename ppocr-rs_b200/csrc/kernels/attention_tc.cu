@@ -19,9 +19,9 @@
 // accumulator in TMEM is rarely rescaled.
 //
 // Bound: the tensor cores, but for the pipeline's gaps.  A prompt of 8,191 tokens,
-// 16 heads on 2 KV heads of 128, causal: 258 us (1,065 TFLOP/s), 7 ragged prompts of up
-// to 2,500, 32 heads on 8: 163 us; the products alone, without softmax, take 187 us
-// of the 258, since S reads both operands from shared memory.  Tried: tiles of
+// 16 heads on 2 KV heads of 128, causal: 257 us (1,070 TFLOP/s), 7 ragged prompts of up
+// to 2,500, 32 heads on 8: 157 us; the products alone, without softmax, take 187 us
+// of the 257, since S reads both operands from shared memory.  Tried: tiles of
 // 64 keys with two buffers of S, 279 to 336 us (products of N = 64 wait for
 // shared memory); two softmax warpgroups to a tile, 290; outputs staged through
 // shared memory before they leave, slower by 2,000 cycles a tile.

@@ -11,10 +11,10 @@
 // Both kernels are bound by HBM: values are read once in their own type (the
 // second look at a page's new values, after its maximum is known, hits
 // registers or L1) and written once in 8 bits, or the reverse.  9,096 tokens of 8
-// heads of 128 in BF16, pages of 32: append 22 us (2.5 TB/s), read 15 us (3.7); the
+// heads of 128 in BF16, pages of 32: append 20 us (2.8 TB/s), read 16 us (3.6); the
 // dozen instructions per value of the exact rounding (a branch to 64-bit
 // arithmetic for near ties: 33 us) and one wave of loads are what is left.  256
-// single tokens of 4 heads of 64 in FP32: 9.5 us, a launch and three dependent
+// single tokens of 4 heads of 64 in FP32: 9.7 us, a launch and three dependent
 // reads (offsets, table, page).
 #include "seq_common.cuh"
 
