@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
             }
         };
         // A new maximum, or a V scale whose product with a weight of 1 would pass FP16.
-        if (__any_sync(0xffffffffu, t0 > m0 || t1 > m1 || fmaxf(sv[0], sv[1]) * units > kMost)) {
+        if (__any_sync(0xffffffffu, t0 > m0 || t1 > m1 || fmaxf(fabsf(sv[0]), fabsf(sv[1])) * units > kMost)) {
             auto rescale = [&](int head, float& unit, int& e, int next, float back) {
 #pragma unroll
                 for (int j = 0; j < KS; ++j) {
@@ -395,8 +395,8 @@ __global__ void __launch_bounds__(kThreads, 3) attention_cached_kernel(CachedAtt
                 if (next > e) rescale(head, unit, e, next, power(max(e - next, -126)));   // what 2^-126 leaves of a sum counts for nothing
             };
             static_assert(kPair == 2, "the largest products of two tiles");
-            cover(fmaxf(fmaxf(s[0][0], s[0][2]) * sv[0], fmaxf(s[1][0], s[1][2]) * sv[1]), e0, unit0, 0);
-            cover(fmaxf(fmaxf(s[0][1], s[0][3]) * sv[0], fmaxf(s[1][1], s[1][3]) * sv[1]), e1, unit1, 1);
+            cover(fmaxf(fmaxf(s[0][0], s[0][2]) * fabsf(sv[0]), fmaxf(s[1][0], s[1][2]) * fabsf(sv[1])), e0, unit0, 0);
+            cover(fmaxf(fmaxf(s[0][1], s[0][3]) * fabsf(sv[0]), fmaxf(s[1][1], s[1][3]) * fabsf(sv[1])), e1, unit1, 1);
             units = fmaxf(unit0, unit1);
 #pragma unroll
             for (int h = 0; h < kPair; ++h) {

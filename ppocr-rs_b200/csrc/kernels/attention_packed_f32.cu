@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS)
     const int keys0 = at.keys_of(min(n0, rows - 1)), keys1 = at.keys_of(min(n0 + 8, rows - 1));
     const int sure = __reduce_min_sync(0xffffffffu, (unsigned)min(keys0, keys1));   // keys every row of the warp sees
     const int most = n0 - r < rows ? (int)__reduce_max_sync(0xffffffffu, (unsigned)max(keys0, keys1)) : 0;
-    // So are rows whose factor and scale might overflow with a key's.
+    // Rows whose factor, scale and a key's factor might overflow are left to attend_row too.
     auto factor = [&](int n) { return fq[n] * scale < power(82) ? fq[n] * scale : NAN; };
     const float f0 = factor(n0), f1 = factor(n0 + 8);
     float o[DT][4];

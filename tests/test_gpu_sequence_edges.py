@@ -520,3 +520,21 @@ def test_packed_no_numbers_behind_a_sequence_cost_nothing(gpu, d, causal):
         outs.append(torch.cat(one))
     assert torch.equal(*outs)
     assert max(times[2:]) < 20 * max(times[:2])   # 84 ms against 0.06 when they did
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_cached_scales_of_either_sign(gpu, dtype):
+    """A cache of the caller's own making may hold negative scales."""
+    g = ops.rng(70)
+    lengths, page, d = [100, 900, 17], 16, 64
+    cache, table = ops.make_cache(g, lengths, 2, d, page)
+    for x in (cache.k_scales, cache.v_scales):
+        x *= torch.where(torch.rand(x.shape, device="cuda", generator=g) < 0.5, -1.0, 1.0)
+    cache.v_scales[table[0, :3].long()] = -cache.v_scales[table[0, :3].long()].abs()
+    q = torch.randn(3, 4, d, device="cuda", generator=g).to(DT[dtype])
+    out = cached(gpu, cache, q, lengths, table)
+    for i, n in enumerate(lengths):
+        k, v = ops.cache_values(cache, table, i, n, page)
+        ref, mag, prod = ops.attend(q[i:i + 1].double(), k, v, d ** -0.5)
+        tol = ops.tolerance(ref, mag, prod, d, n, dtype, 2.0 ** -11 if dtype == "bf16" else 2.0 ** -20)
+        ops.check(out[i:i + 1], ref, tol + n * 2.0 ** -31 * v.abs().max())
